@@ -239,6 +239,29 @@ KVB_API int kvb_w8a8_scaled_mm_act_allgather(const int8_t* a, const int8_t* b_sh
                                              int64_t M, int64_t N_shard, int64_t K, int act, void* const* out_ptrs,
                                              int world, int rank, int64_t ldo, int out_dtype, void* stream);
 
+/* ---------------------------------------------------------------- rotary position embedding */
+
+/*
+ * Per-head RMSNorm (optional) and rotary position embedding of queries and keys in one pass (no
+ * reference counterpart; stands before kvb_batched_prefill_attention).
+ *   y = x * rsqrt(mean(x^2) + eps) * weight            (per head of head_dim elements; only with a weight)
+ *   (y_i, y_j) -> (y_i c_n - y_j s_n, y_j c_n + y_i s_n),  n < rotary_dim / 2
+ * with (i, j) = (n, n + rotary_dim / 2), or (2 n, 2 n + 1) when `interleaved`; elements rotary_dim ..
+ * head_dim pass.  (c, s) is row positions[token] of cos_sin [max_positions, rotary_dim] float32:
+ * rotary_dim / 2 cosines, then as many sines.  float32 arithmetic, one rounding at the end.
+ * q [num_tokens, num_q_heads, head_dim] and k [num_tokens, num_kv_heads, head_dim] of `dtype`
+ * (KVB_F32 / F16 / BF16) with the given token and head strides (elements; the head's elements are
+ * contiguous), so both may be views of one fused projection.  positions: KVB_I32 or KVB_I64; a
+ * position outside [0, max_positions) gives NaN heads and sets bit 1 of kvb_device_status.
+ * q_weight / k_weight [head_dim] of `dtype`, or NULL (no norm).  q_out / k_out: contiguous, of
+ * `dtype`, not overlapping the inputs.  head_dim and rotary_dim even, rotary_dim <= head_dim <= 1024.
+ */
+KVB_API int kvb_qk_norm_rope(const void* q, const void* k, int dtype, int64_t q_token_stride, int64_t q_head_stride,
+                             int64_t k_token_stride, int64_t k_head_stride, const void* positions, int positions_dtype,
+                             const float* cos_sin, int64_t max_positions, int rotary_dim, int interleaved,
+                             const void* q_weight, const void* k_weight, float eps, int64_t num_tokens, int num_q_heads,
+                             int num_kv_heads, int head_dim, void* q_out, void* k_out, void* stream);
+
 /* ---------------------------------------------------------------- paged KV-cache writes */
 
 /*
@@ -278,6 +301,30 @@ KVB_API int kvb_kv_cache_write(const void* key, const void* value, const void* k
                                void* k_cache_out, void* v_cache_out, const void* positions, int index_dtype,
                                int per_batch, int dtype, int64_t batch, int64_t heads, int64_t max_seq_len,
                                int64_t write_len, int64_t head_dim, void* stream);
+
+/*
+ * kvb_qk_norm_rope on the way into a paged KV cache (no reference counterpart; slot placement as
+ * paged_kv_cache_update.py:27-30): the normalised and rotated keys and the values
+ * v [num_tokens, num_kv_heads, head_dim] are stored in slot slot_mapping[token] (KVB_I32 or KVB_I64)
+ * of k_cache / v_cache [num_blocks, block_size, num_kv_heads, head_dim], and the normalised and
+ * rotated queries in q_out.  cache_dtype: `dtype`, or KVB_E4M3 with float32 k_scale / v_scale
+ * [num_kv_heads]: code = e4m3(clamp(y / scale[h], +-448)), quantised from the float32 value.  The
+ * blocks of each cache may be further apart than they are long (k_block_stride / v_block_stride,
+ * elements), as in a cache that holds keys and values of a block side by side.  A token with a
+ * negative slot is kept out of the cache and its query is rotated all the same; a slot at or past
+ * num_blocks * block_size is skipped and sets bit 1 of kvb_device_status; a token whose position is
+ * out of range is kept out of the cache, gives NaN queries and sets the same bit.  Slots must be
+ * distinct: of two tokens with one slot, either may be stored in each vector of the row.
+ */
+KVB_API int kvb_rope_paged_kv_append(const void* q, const void* k, const void* v, int dtype, int64_t q_token_stride,
+                                     int64_t q_head_stride, int64_t k_token_stride, int64_t k_head_stride,
+                                     int64_t v_token_stride, int64_t v_head_stride, const void* positions,
+                                     int positions_dtype, const void* slot_mapping, int slot_dtype, const float* cos_sin,
+                                     int64_t max_positions, int rotary_dim, int interleaved, const void* q_weight,
+                                     const void* k_weight, float eps, int64_t num_tokens, int num_q_heads,
+                                     int num_kv_heads, int head_dim, void* k_cache, void* v_cache, int cache_dtype,
+                                     int block_size, int64_t num_blocks, int64_t k_block_stride, int64_t v_block_stride,
+                                     const float* k_scale, const float* v_scale, void* q_out, void* stream);
 
 /* ---------------------------------------------------------------- paged decode attention */
 
@@ -379,6 +426,53 @@ KVB_API int kvb_batched_prefill_attention_variant(const void* q, const void* k, 
                                                   int64_t total_q, int64_t total_kv, int num_q_heads,
                                                   int num_kv_heads, int head_dim, float softmax_scale, void* out,
                                                   int variant, void* stream);
+
+/* Bytes of workspace kvb_paged_prefill_attention needs (the partial results of items cut between CTAs). */
+KVB_API size_t kvb_paged_prefill_attention_workspace_size(int head_dim);
+
+/*
+ * Causal attention of a ragged batch of chunks of new tokens over a paged KV cache (no reference
+ * counterpart: batched_prefill_attention.py:30-73 over the cache of paged_attention_v1.py:27-92).
+ * q [total_q, num_q_heads, head_dim] (q_dtype; q_token_stride elements between tokens, heads
+ * contiguous); request b owns query rows [qo_indptr[b], qo_indptr[b + 1]) (int32, device) and holds
+ * seq_lens[b] tokens (KVB_I32 / KVB_I64) in the cache, the chunk's own among them, so its query i
+ * stands at position seq_len - q_len + i and attends keys 0 .. that position; a query at a negative
+ * position attends nothing (output 0, log-sum-exp -inf).  One token a request is decoding; chunks of
+ * any lengths may be mixed.  k_cache / v_cache [num_blocks, block_size, num_kv_heads, head_dim]
+ * (block strides in elements): q_dtype, or KVB_E4M3 with float32 k_scale / v_scale [num_kv_heads].
+ * Token t of request b is row t % block_size of block block_table[b * bt_stride + t / block_size];
+ * table entries past a request's last token, and cache rows past it, are not read into the result
+ * (they may hold anything).  Query head h reads KV head h / (num_q_heads / num_kv_heads).
+ * out [total_q, num_q_heads, head_dim] of q_dtype; lse [total_q, num_q_heads] float32 or NULL: the
+ * natural-log sum of exp of the scaled logits.  Query rows that no request owns are left as they
+ * were.  max_seq_len >= every seq_len.  A request whose lengths lie outside the tensors is skipped
+ * (bit 2 of kvb_device_status); a block-table entry out of range counts as zero keys and values and
+ * sets bit 1.  Float32 softmax state; parts of one row are joined in a fixed order, so equal inputs
+ * give equal outputs.  head_dim a multiple of 8, at most 128.  workspace: >=
+ * kvb_paged_prefill_attention_workspace_size() bytes, 256-byte aligned, not shared with a launch that
+ * may run at the same time.
+ */
+KVB_API int kvb_paged_prefill_attention(const void* q, int q_dtype, int64_t q_token_stride, const void* k_cache,
+                                        const void* v_cache, int cache_dtype, int64_t k_block_stride,
+                                        int64_t v_block_stride, const float* k_scale, const float* v_scale,
+                                        const int32_t* qo_indptr, const void* seq_lens, int seq_lens_dtype,
+                                        const int32_t* block_table, int64_t bt_stride, int batch, int64_t total_q,
+                                        int num_q_heads, int num_kv_heads, int head_dim, int block_size,
+                                        int64_t num_blocks, int64_t max_seq_len, float sm_scale, void* out, float* lse,
+                                        void* workspace, size_t workspace_bytes, void* stream);
+/*
+ * The same with the kernel chosen (test hook, no reference counterpart): variant 0 = automatic, 1 =
+ * the mma.sync kernel, 2 = the tcgen05 kernel (KVB_E_SHAPE where it does not apply).
+ */
+KVB_API int kvb_paged_prefill_attention_variant(const void* q, int q_dtype, int64_t q_token_stride, const void* k_cache,
+                                                const void* v_cache, int cache_dtype, int64_t k_block_stride,
+                                                int64_t v_block_stride, const float* k_scale, const float* v_scale,
+                                                const int32_t* qo_indptr, const void* seq_lens, int seq_lens_dtype,
+                                                const int32_t* block_table, int64_t bt_stride, int batch, int64_t total_q,
+                                                int num_q_heads, int num_kv_heads, int head_dim, int block_size,
+                                                int64_t num_blocks, int64_t max_seq_len, float sm_scale, void* out,
+                                                float* lse, int variant, void* workspace, size_t workspace_bytes,
+                                                void* stream);
 
 /*
  * Allocation-free variant of kvb_paged_attention (no counterpart in the reference).

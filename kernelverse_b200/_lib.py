@@ -50,6 +50,16 @@ SIGNATURES = {
     "kvb_batched_prefill_attention": (_I, [_P, _P, _P, _I, _P, _P, _I, _I64, _I64, _I, _I, _I, _F, _P, _P]),
     "kvb_batched_prefill_attention_variant": (_I, [_P, _P, _P, _I, _P, _P, _I, _I64, _I64, _I, _I, _I, _F, _P, _I,
                                                    _P]),
+    "kvb_qk_norm_rope": (_I, [_P, _P, _I, _I64, _I64, _I64, _I64, _P, _I, _P, _I64, _I, _I, _P, _P, _F, _I64, _I,
+                             _I, _I, _P, _P, _P]),
+    "kvb_rope_paged_kv_append": (_I, [_P, _P, _P, _I, _I64, _I64, _I64, _I64, _I64, _I64, _P, _I, _P, _I, _P, _I64,
+                                     _I, _I, _P, _P, _F, _I64, _I, _I, _I, _P, _P, _I, _I, _I64, _I64, _I64, _P, _P,
+                                     _P, _P]),
+    "kvb_paged_prefill_attention": (_I, [_P, _I, _I64, _P, _P, _I, _I64, _I64, _P, _P, _P, _P, _I, _P, _I64, _I,
+                                        _I64, _I, _I, _I, _I, _I64, _I64, _F, _P, _P, _P, _SZ, _P]),
+    "kvb_paged_prefill_attention_variant": (_I, [_P, _I, _I64, _P, _P, _I, _I64, _I64, _P, _P, _P, _P, _I, _P, _I64,
+                                                _I, _I64, _I, _I, _I, _I, _I64, _I64, _F, _P, _P, _I, _P, _SZ, _P]),
+    "kvb_paged_prefill_attention_workspace_size": (_SZ, [_I]),
     "kvb_paged_attention_noalloc": (_I, [_P, _I, _P, _P, _I, _P, _P, _P, _I, _P, _I64, _I, _I, _I, _I, _I, _I64, _I64,
                                          _F, _P, _P, _I, _I, _P, _I, _P, _P, _P, _I, _P]),
 }

@@ -10,6 +10,8 @@ tensors through the GPU kernel.
 """
 from __future__ import annotations
 
+from contextlib import nullcontext
+from functools import lru_cache
 from typing import Optional, Tuple
 
 import torch
@@ -48,6 +50,18 @@ def _ptr(t: Optional[torch.Tensor]):
 
 def _stream(dev: torch.device) -> int:
     return torch.cuda.current_stream(dev).cuda_stream
+
+@lru_cache(maxsize=None)
+def _paged_prefill_workspace(head_dim: int) -> int:
+    return _lib.lib().kvb_paged_prefill_attention_workspace_size(head_dim)
+
+
+def _on(dev: torch.device):
+    """Makes ``dev`` the current device for a launch; nothing to do where it already is."""
+    return _HERE if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+_HERE = nullcontext()
 
 
 _workspaces = {}
@@ -313,6 +327,140 @@ def paged_fp8_kv_write(x_new: torch.Tensor, cache: torch.Tensor, slot_mapping: t
     return cache
 
 
+# --------------------------------------------------------------------------- rotary position embedding
+def rope_cos_sin(max_positions: int, rotary_dim: int, base: float = 10000.0, device=None) -> torch.Tensor:
+    """The cos/sin table that :func:`qk_norm_rope` and :func:`rope_paged_kv_append` read: float32
+    ``[max_positions, rotary_dim]``, row p the cosines of ``p * base^(-2n / rotary_dim)``, n < rotary_dim / 2,
+    then their sines.  Angles are computed in float64 on the host; made once per model."""
+    if rotary_dim < 0 or rotary_dim % 2 or max_positions < 0:
+        raise ValueError("rope_cos_sin: max_positions >= 0 and an even rotary_dim >= 0")
+    freq = torch.pow(torch.tensor(float(base), dtype=torch.float64),
+                     -torch.arange(0, rotary_dim, 2, dtype=torch.float64) / max(rotary_dim, 1))
+    angle = torch.arange(max_positions, dtype=torch.float64)[:, None] * freq
+    table = torch.cat((angle.cos(), angle.sin()), 1).to(torch.float32)
+    return table if device is None else table.to(device)
+
+
+def _heads(what: str, name: str, t: torch.Tensor) -> torch.Tensor:
+    """A [tokens, heads, head_dim] tensor whose last dimension is contiguous (views of a fused
+    projection stay views)."""
+    if t.dim() != 3:
+        raise ValueError(f"{what}: {name} must be [tokens, heads, head_dim]")
+    return t if t.stride(2) == 1 else t.contiguous()
+
+
+def _rope_args(what, q, k, positions, cos_sin, q_weight, k_weight):
+    """Checks shared by the two rope entry points; returns (q, k, positions, cos_sin, weights)."""
+    q, k = _heads(what, "q", q), _heads(what, "k", k)
+    t, hq, d = q.shape
+    if k.shape[0] != t or k.shape[2] != d:
+        raise ValueError(f"{what}: q and k must have the same tokens and head_dim")
+    if k.dtype != q.dtype:
+        raise TypeError(f"{what}: q and k must share a dtype")
+    if positions.dim() != 1 or positions.shape[0] != t:
+        raise ValueError(f"{what}: positions must be [tokens]")
+    if cos_sin.dim() != 2 or cos_sin.dtype != torch.float32:
+        raise TypeError(f"{what}: cos_sin must be float32 [max_positions, rotary_dim]")
+    for w in (q_weight, k_weight):
+        if w is not None and (w.shape != (d,) or w.dtype != q.dtype):
+            raise ValueError(f"{what}: norm weights must be [head_dim] of q's dtype")
+    return (q, k, positions.contiguous(), cos_sin.contiguous(), None if q_weight is None else q_weight.contiguous(),
+            None if k_weight is None else k_weight.contiguous())
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor,
+                 q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                 interleaved: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Per-head RMSNorm (where a weight is given) and rotary position embedding of queries and keys.
+
+    q [T, Hq, D] and k [T, Hkv, D] (float32, float16 or bfloat16; token and head strides are free, so
+    both may be views of one fused projection); positions [T] int32 / int64; cos_sin float32
+    [max_positions, R] (:func:`rope_cos_sin`), R <= D: the first R elements of a head rotate, paired
+    as halves (n, n + R/2) or, ``interleaved``, as neighbours (2n, 2n + 1).  float32 arithmetic with one
+    rounding.  Returns new contiguous ``(q_out, k_out)``, as :func:`batched_prefill_attention` takes
+    them.  A position outside the table gives NaN heads and sets device status bit 1."""
+    dev = _cuda(q, k, positions, cos_sin, q_weight, k_weight)
+    q, k, positions, cos_sin, q_weight, k_weight = _rope_args("qk_norm_rope", q, k, positions, cos_sin, q_weight, k_weight)
+    t, hq, d = q.shape
+    hkv = k.shape[1]
+    with _on(dev):
+        q_out = torch.empty((t, hq, d), dtype=q.dtype, device=dev)
+        k_out = torch.empty((t, hkv, d), dtype=q.dtype, device=dev)
+        call("kvb_qk_norm_rope", q.data_ptr(), k.data_ptr(), kvb_dtype(q.dtype), q.stride(0), q.stride(1), k.stride(0),
+             k.stride(1), positions.data_ptr(), _index_dtype(positions), cos_sin.data_ptr(), cos_sin.shape[0],
+             cos_sin.shape[1], 1 if interleaved else 0, _ptr(q_weight), _ptr(k_weight), float(eps), t, hq, hkv, d,
+             q_out.data_ptr(), k_out.data_ptr(), _stream(dev))
+    return q_out, k_out
+
+
+def _paged_blocks(what: str, name: str, cache: torch.Tensor) -> int:
+    """Checks a paged cache that is used in place ([num_blocks, block_size, Hkv, D], each block
+    contiguous) and returns its block stride in elements."""
+    if cache.dim() != 4:
+        raise ValueError(f"{what}: {name} must be [num_blocks, block_size, num_kv_heads, head_dim]")
+    nb, bs, h, d = cache.shape
+    want = (h * d, d, 1)
+    if any(n > 1 and s != w for n, s, w in zip((bs, h, d), cache.stride()[1:], want)):
+        raise ValueError(f"{what}: the blocks of {name} must be contiguous")
+    return cache.stride(0) if nb > 1 else bs * h * d
+
+
+def _cache_scales(what, cache_dtype, hkv, k_scale, v_scale):
+    """float32 [Hkv] scales of an e4m3 cache, or (None, None) for a cache that takes none."""
+    if cache_dtype != _lib.E4M3:
+        if k_scale is not None or v_scale is not None:
+            raise ValueError(f"{what}: scales belong to e4m3 caches")
+        return None, None
+    if k_scale is None or v_scale is None:
+        raise ValueError(f"{what}: an e4m3 cache needs k_scale and v_scale")
+    if k_scale.numel() != hkv or v_scale.numel() != hkv:
+        raise ValueError(f"{what}: k_scale and v_scale must have one entry per KV head")
+    return k_scale.to(torch.float32).contiguous(), v_scale.to(torch.float32).contiguous()
+
+
+def rope_paged_kv_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                         slot_mapping: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor,
+                         k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None,
+                         q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None,
+                         eps: float = 1e-6, interleaved: bool = False) -> torch.Tensor:
+    """:func:`qk_norm_rope` on the way into a paged cache: the keys go, normalised and rotated, and the
+    values as they are, into slot ``slot_mapping[t]`` of the caches (in place), and the rotated queries
+    [T, Hq, D] come back.
+
+    Caches [num_blocks, block_size, Hkv, D] of q's dtype, or e4m3 codes (float8_e4m3fn or uint8) with
+    float32 ``k_scale`` / ``v_scale`` [Hkv]: ``code = e4m3(clamp(x / scale[h], +-448))``, quantised from the
+    float32 value.  Blocks may lie apart (``kv[:, 0]`` and ``kv[:, 1]`` of one tensor) but must be contiguous.
+    A negative slot keeps its token out of the cache; slots must be distinct.  Slots or positions out of
+    range set device status bit 1."""
+    what = "rope_paged_kv_append"
+    dev = _cuda(q, k, v, k_cache, v_cache, slot_mapping, positions, cos_sin, k_scale, v_scale, q_weight, k_weight)
+    q, k, positions, cos_sin, q_weight, k_weight = _rope_args(what, q, k, positions, cos_sin, q_weight, k_weight)
+    v = _heads(what, "v", v)
+    t, hq, d = q.shape
+    hkv = k.shape[1]
+    if v.shape != k.shape or v.dtype != k.dtype:
+        raise ValueError(f"{what}: v must have k's shape and dtype")
+    if v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype or k_cache.shape[2:] != (hkv, d):
+        raise ValueError(f"{what}: caches must both be [num_blocks, block_size, num_kv_heads, head_dim]")
+    cdt = _cache_kvb_dtype(k_cache)
+    if cdt != _lib.E4M3 and k_cache.dtype != q.dtype:
+        raise TypeError(f"{what}: caches hold q's dtype or e4m3 codes")
+    ks, vs = _paged_blocks(what, "k_cache", k_cache), _paged_blocks(what, "v_cache", v_cache)
+    if slot_mapping.dim() != 1 or slot_mapping.shape[0] != t:
+        raise ValueError(f"{what}: slot_mapping must be [tokens]")
+    with _on(dev):
+        k_scale, v_scale = _cache_scales(what, cdt, hkv, k_scale, v_scale)
+        slot_mapping = slot_mapping.contiguous()
+        q_out = torch.empty((t, hq, d), dtype=q.dtype, device=dev)
+        call("kvb_rope_paged_kv_append", q.data_ptr(), k.data_ptr(), v.data_ptr(), kvb_dtype(q.dtype), q.stride(0),
+             q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1), positions.data_ptr(), _index_dtype(positions),
+             slot_mapping.data_ptr(), _index_dtype(slot_mapping), cos_sin.data_ptr(), cos_sin.shape[0], cos_sin.shape[1],
+             1 if interleaved else 0, _ptr(q_weight), _ptr(k_weight), float(eps), t, hq, hkv, d, k_cache.data_ptr(),
+             v_cache.data_ptr(), cdt, k_cache.shape[1], k_cache.shape[0], ks, vs, _ptr(k_scale), _ptr(v_scale),
+             q_out.data_ptr(), _stream(dev))
+    return q_out
+
+
 # --------------------------------------------------------------------------- decode attention
 def _cache_kvb_dtype(t: torch.Tensor) -> int:
     if t.dtype in (torch.uint8, torch.float8_e4m3fn):
@@ -435,6 +583,67 @@ def batched_prefill_attention(q, k, v, qo_indptr, kv_indptr, softmax_scale: Opti
          _ptr(kv_indptr), qo_indptr.numel() - 1, tq, tkv, hq, hkv, d, float(scale), _ptr(out), int(_variant),
          _stream(dev))
     return out
+
+
+def paged_prefill_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, qo_indptr: torch.Tensor,
+                            seq_lens: torch.Tensor, block_table: torch.Tensor, scale: Optional[float] = None,
+                            k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None,
+                            max_seq_len: Optional[int] = None, return_lse: bool = False,
+                            out: Optional[torch.Tensor] = None, _variant: int = 0):
+    """Causal attention of a ragged batch of chunks of new tokens over a paged KV cache.
+
+    q [total_q, Hq, D]; request b owns rows ``qo_indptr[b]:qo_indptr[b + 1]`` (int32 [B + 1]) and holds
+    ``seq_lens[b]`` tokens in the cache, the chunk's own among them (:func:`rope_paged_kv_append` puts
+    them there), so its query i stands at position ``seq_len - q_len + i`` and attends keys 0 .. that
+    position.  One token a request is a decode step, a few check drafted tokens, many prefill a prompt;
+    a batch may mix them.  Caches [num_blocks, block_size, Hkv, D] of q's dtype, or e4m3 codes
+    (float8_e4m3fn or uint8) with float32 ``k_scale`` / ``v_scale`` [Hkv]; block_table int32 [B, max_blocks].
+    Logits are scaled by ``scale`` (default D^-0.5); float32 softmax.  ``max_seq_len`` (default: what the
+    block table holds) bounds every seq_len.
+
+    Returns [total_q, Hq, D] in q's dtype (``out`` when given), and with ``return_lse`` the natural-log
+    sums of exp [total_q, Hq] float32.  A query that sees no key (q_len > seq_len) gives 0 and -inf; rows
+    past the last request are left as they were.  Equal inputs give equal outputs."""
+    what = "paged_prefill_attention"
+    dev = _cuda(q, k_cache, v_cache, qo_indptr, seq_lens, block_table, k_scale, v_scale, out)
+    if q.dim() != 3:
+        raise ValueError(f"{what}: q must be [total_q, num_q_heads, head_dim]")
+    tq, hq, d = q.shape
+    if v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype or k_cache.dim() != 4 or k_cache.shape[3] != d:
+        raise ValueError(f"{what}: caches must both be [num_blocks, block_size, num_kv_heads, head_dim]")
+    nb, bs, hkv, _ = k_cache.shape
+    cdt = _cache_kvb_dtype(k_cache)
+    if cdt != _lib.E4M3 and k_cache.dtype != q.dtype:
+        raise TypeError(f"{what}: caches hold q's dtype or e4m3 codes")
+    ks, vs = _paged_blocks(what, "k_cache", k_cache), _paged_blocks(what, "v_cache", v_cache)
+    if qo_indptr.dtype != torch.int32 or block_table.dtype != torch.int32:
+        raise TypeError(f"{what}: qo_indptr and block_table must be int32")
+    b = seq_lens.shape[0] if seq_lens.dim() == 1 else -1
+    if qo_indptr.dim() != 1 or qo_indptr.shape[0] != b + 1 or block_table.dim() != 2 or block_table.shape[0] != b:
+        raise ValueError(f"{what}: qo_indptr [batch + 1], seq_lens [batch], block_table [batch, max_blocks]")
+    if max_seq_len is None:
+        max_seq_len = block_table.shape[1] * bs
+    scale = d ** -0.5 if scale is None else scale
+    if q.stride(2) != 1 or q.stride(1) != d or (q.stride(0) * q.element_size()) % 16 or q.data_ptr() % 16:
+        q = q.contiguous()
+    with _on(dev):
+        k_scale, v_scale = _cache_scales(what, cdt, hkv, k_scale, v_scale)
+        qo_indptr, seq_lens = qo_indptr.contiguous(), seq_lens.contiguous()
+        if block_table.stride(1) != 1 or block_table.stride(0) < block_table.shape[1]:
+            block_table = block_table.contiguous()
+        if out is None:
+            out = torch.empty((tq, hq, d), dtype=q.dtype, device=dev)
+        elif out.shape != (tq, hq, d) or out.dtype != q.dtype or not out.is_contiguous():
+            raise ValueError(f"{what}: out must be a contiguous tensor of q's shape and dtype")
+        lse = torch.empty((tq, hq), dtype=torch.float32, device=dev) if return_lse else None
+        # per call, from the caching allocator: calls on other streams and captured graphs do not share it
+        ws = torch.empty(_paged_prefill_workspace(d), dtype=torch.uint8, device=dev)
+        call("kvb_paged_prefill_attention_variant", q.data_ptr(), kvb_dtype(q.dtype), q.stride(0), k_cache.data_ptr(),
+             v_cache.data_ptr(), cdt, ks, vs, _ptr(k_scale), _ptr(v_scale), qo_indptr.data_ptr(), seq_lens.data_ptr(),
+             _index_dtype(seq_lens), block_table.data_ptr(), block_table.stride(0), b, tq, hq, hkv, d, bs, nb,
+             int(max_seq_len), float(scale), out.data_ptr(), _ptr(lse), int(_variant), ws.data_ptr(), ws.numel(),
+             _stream(dev))
+    return (out, lse) if return_lse else out
 
 
 _FLASH_DECODE_INDEX = {}

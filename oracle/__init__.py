@@ -13,4 +13,4 @@ running the reference's own ``Model.forward`` on CPU (torch 2.11.0), and
 ``tests/test_oracle_numerics.py`` checks the e4m3 encoder against the format
 definition and torch's cast.
 """
-from . import attention, gemm, kv_cache, numerics, quant, rmsnorm  # noqa: F401
+from . import attention, gemm, kv_cache, numerics, quant, rmsnorm, rope  # noqa: F401

@@ -228,3 +228,35 @@ def batched_prefill_attention(q, k, v, qo_indptr, kv_indptr, num_q_heads: int, n
             p = np.exp(sc - m)
             out[q0:q1, h] = (p @ vv) / p.sum(axis=1, keepdims=True)
     return out.astype(np.float32)
+
+
+def paged_prefill_attention(q, k_cache, v_cache, qo_indptr, seq_lens, block_table, scale: float):
+    """Chunks of new tokens over a paged cache of float64 values ``[nb, bs, Hkv, D]``: query i of
+    request b is at position ``seq_len - q_len + i`` and sees keys ``<=`` it; a query at a negative
+    position gives 0 and a log-sum-exp of -inf.  Returns float64 ``(out [Tq, Hq, D], lse [Tq, Hq],
+    weight [Tq, Hq, D], reach [Tq, Hq])``: ``weight`` is the same average of ``|v|`` and ``reach`` the
+    largest ``|scale| sum_d |q_d k_d|`` of the row, which rounding errors are relative to."""
+    qf = np.asarray(q, np.float64)
+    tq, hq, d = qf.shape
+    grp = hq // k_cache.shape[2]
+    out, weight = np.zeros(qf.shape), np.zeros(qf.shape)
+    lse, reach = np.full((tq, hq), -np.inf), np.zeros((tq, hq))
+    for b in range(len(seq_lens)):
+        q0, q1, L = int(qo_indptr[b]), int(qo_indptr[b + 1]), int(seq_lens[b])
+        if L == 0 or q1 == q0:
+            continue
+        k = np.asarray(gather_sequence(k_cache, block_table[b], L), np.float64)
+        v = np.asarray(gather_sequence(v_cache, block_table[b], L), np.float64)
+        for i in range(q0, q1):
+            n = L - (q1 - q0) + (i - q0) + 1            # keys the query sees
+            if n <= 0:
+                continue
+            for h in range(hq):
+                kk, vv = k[:n, h // grp], v[:n, h // grp]
+                z = (kk @ qf[i, h]) * scale
+                p = np.exp(z - z.max())
+                lse[i, h] = z.max() + np.log(p.sum())
+                out[i, h] = p @ vv / p.sum()
+                weight[i, h] = p @ np.abs(vv) / p.sum()
+                reach[i, h] = (np.abs(kk) @ np.abs(qf[i, h])).max() * abs(scale)
+    return out, lse, weight, reach
