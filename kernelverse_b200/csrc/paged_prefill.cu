@@ -14,6 +14,7 @@
 // accuracy), online softmax in the log2 domain.  e4m3 codes become the query's type on their way
 // into shared memory (exactly: both 16-bit types hold every code) and the scales go into the logit
 // scale and the output.
+#include <algorithm>
 #include <cmath>
 #include <type_traits>
 
@@ -23,6 +24,9 @@
 #include "paged_prefill.cuh"
 
 namespace kvb {
+
+bool paged_prefill_tc_takes(const PagedArgs& a, int q_dtype, int cache_dtype);
+int paged_prefill_tcgen05(PagedArgs& a, int q_dtype, int cache_dtype, void* ws, int sms, cudaStream_t st);
 
 namespace {
 
@@ -67,7 +71,7 @@ __global__ void __launch_bounds__(kPpThreads, 2) paged_prefill_kernel(const __gr
   __shared__ int2 page[2][BK];                       // {block, row in it} of a tile's keys; block -1: nothing there
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
   const int D = a.D;
-  const PgTiles tiles{kPpRows, BK, a.group};
+  const PgTiles tiles{kPpRows, BK, a.group, 0, 0};
 
   // Padding columns [D, DP) of every shared row are zero for the whole kernel (the copies never
   // write them), so they add nothing to Q K^T.
@@ -442,7 +446,7 @@ int paged_sms() {
 
 extern "C" size_t kvb_paged_prefill_attention_workspace_size(int head_dim) {
   if (head_dim <= 0 || head_dim > 128) return 256;
-  return pg_workspace_bytes(kPgMaxCtas, kPpRows, head_dim);
+  return std::max(pg_workspace_bytes(kPgMaxCtas, kPpRows, head_dim), pg_workspace_bytes(kPgMaxCtas / 2, 256, head_dim));
 }
 
 extern "C" int kvb_paged_prefill_attention_variant(const void* q, int q_dtype, int64_t q_token_stride,
@@ -497,7 +501,9 @@ extern "C" int kvb_paged_prefill_attention_variant(const void* q, int q_dtype, i
       workspace_bytes < kvb_paged_prefill_attention_workspace_size(head_dim))
     return set_error(KVB_E_WORKSPACE, "paged_prefill_attention: %zu bytes of workspace, 256-byte aligned, are needed",
                      kvb_paged_prefill_attention_workspace_size(head_dim));
-  if (variant == 2) return set_error(KVB_E_SHAPE, "paged_prefill_attention: no tcgen05 kernel for this case");
+  const bool tc = paged_prefill_tc_takes(a, q_dtype, cache_dtype);
+  if (variant == 2 && !tc) return set_error(KVB_E_SHAPE, "paged_prefill_attention: no tcgen05 kernel for this case");
+  if (tc && variant != 1) return paged_prefill_tcgen05(a, q_dtype, cache_dtype, workspace, sms, st);
   pg_workspace_layout(a, workspace, grid, kPpRows);
   int rc;
   const bool e4 = cache_dtype == KVB_E4M3;

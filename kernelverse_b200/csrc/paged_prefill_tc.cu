@@ -1,0 +1,722 @@
+// Causal attention of chunks of new tokens over a paged KV cache on the 5th-generation tensor cores:
+// 16-bit queries over a cache of their type or of e4m3 codes, head_dim a multiple of 16 in [64, 128].
+// The contract and the mathematics are those of paged_prefill.cu.
+//
+// One persistent CTA per SM works through its share of (request, KV head, row tile) items
+// (paged_prefill.cuh).  The query rows of a KV head's group are packed (row = token x group + head), so
+// each key is read once for the whole group.  Two chains S = Q K^T -> softmax -> O += P V run
+// interleaved, each with 128 rows (TMEM lanes), an S buffer and its O in tensor memory and four softmax
+// warps, so one chain's exponentials overlap the other's products:
+//   wide items (over 128 rows): chain A has rows 0..127 of the tile, chain B rows 128..255, and both
+//     use every K/V tile of 128 keys;
+//   deep items (at most 128 rows: decoding, drafts, the last rows of a prompt): both chains have the
+//     same rows, A takes the even K/V tiles and B the odd ones, and the two results are joined.
+// Roles: warp 0 issues the TMA loads (boxes of whole page runs gathered through the block table);
+// warp 1 owns TMEM and issues the MMAs; warps 2, 3, 12, 13 gather the query rows and turn e4m3 codes
+// into float16 operands; warps 4-7 and 8-11 are the softmax groups of A and B.
+// K and V tiles share one ring of shared-memory slots in the order K_0 V_0 K_1 V_1 ...  A page outside
+// the cache, and pages past the last token, are loaded from an out-of-range block coordinate, which
+// TMA fills with zeros; the rows past the last token inside its page are zeroed in shared memory.
+// e4m3: a row of Q is scaled by a power of two that brings its largest element to [1, 2), so float16
+// holds it whatever bfloat16's range had; P is float16 too.
+// Every mbarrier wait is bounded; on a timeout the roles stop, the producer waits for its own copies,
+// the MMA lane for its MMAs, and the CTA frees its TMEM before exiting.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <mutex>
+#include <type_traits>
+
+#include "kvb_common.cuh"
+#include "kvb_async.cuh"
+#include "paged_prefill.cuh"
+#include "tcgen05.cuh"
+
+namespace kvb {
+namespace {
+
+constexpr int kRows = 128;                 // rows of a chain (TMEM lanes)
+constexpr int kKeys = 128;                 // keys per K/V tile
+constexpr int kTile = 2 * kRows;           // rows of a tile
+constexpr int kThreads = 448;
+constexpr int kHelpers = 128;              // threads of warps 2, 3, 12, 13
+constexpr int kMaxSlots = 8;
+constexpr int kMaxRaw = 4;
+
+template <bool kE4m3, int DC> struct PcLayout {
+  static constexpr uint32_t kOp = DC * kChunkBytes;                // one Q, K or V tile of 16-bit operands
+  static constexpr uint32_t kRaw = kE4m3 ? kKeys * 64u * DC : 0u;  // one K or V tile of codes
+  static constexpr uint32_t kBudget = 224 * 1024;
+  static constexpr int kRawSlots = kE4m3 ? 4 : 0;
+  static constexpr int kFit = (int)((kBudget - 2 * kOp - kRawSlots * kRaw) / kOp);
+  static constexpr int kSlots = kFit < 8 ? kFit : 8;
+  static constexpr uint32_t kQ0 = 0, kKv0 = 2 * kOp, kRaw0 = kKv0 + kSlots * kOp;
+  static constexpr size_t kSmem = kRaw0 + (size_t)kRawSlots * kRaw + 1024;
+  static_assert(kSlots >= 3 && kSlots <= kMaxSlots && kRawSlots <= kMaxRaw, "ring");
+};
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+      ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two) {
+  uint32_t r;
+  const uint16_t v = (uint16_t)two;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(v));
+  return r;
+}
+
+// What every role derives from an item.
+struct PcItem {
+  int row0;        // first row of the tile in its request
+  int rw;          // rows of the request
+  int rows;        // rows of the tile
+  bool wide;
+  int kt0, T;      // key tiles [kt0, kt0 + T)
+  int TA;          // wide: how many of them chain A uses
+  __device__ __forceinline__ PcItem(const PagedArgs& a, const PgItem& it) {
+    rw = it.r.ql * a.group;
+    row0 = it.t * kTile;
+    rows = min(kTile, rw - row0);
+    wide = rows > kRows;
+    const int off = (it.r.kl - it.r.ql) * a.group;
+    const int xb = off + row0 + rows - 1;                       // position of the last row x group
+    const int nb = xb < 0 ? 1 : xb / (a.group * kKeys) + 1;     // key tiles of the tile (one where nothing is seen)
+    if (wide) {
+      kt0 = it.j0;
+      T = it.j1 - it.j0;
+      const int xa = off + row0 + kRows - 1;
+      const int na = xa < 0 ? 0 : xa / (a.group * kKeys) + 1;
+      TA = max(1, min(T, na - kt0));                            // (a tile that it sees nothing of keeps the chains in step)
+    } else {
+      kt0 = 2 * it.j0;
+      T = min(2 * (it.j1 - it.j0), nb - kt0);
+      TA = 0;
+    }
+  }
+  // tiles of chain c, the first one and the step to the next
+  __device__ __forceinline__ int count(int c) const { return wide ? (c ? T : TA) : (T - c + 1) >> 1; }
+};
+
+template <typename T, bool kE4m3, int DC>
+__global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __grid_constant__ CUtensorMap tk,
+                                                                       const __grid_constant__ CUtensorMap tv,
+                                                                       const __grid_constant__ PagedArgs a, const int box) {
+  using L = PcLayout<kE4m3, DC>;
+  constexpr bool kBf = !kE4m3 && std::is_same<T, __nv_bfloat16>::value;   // type of the operands
+  // float16 has few exponents: P is held 2^7 larger there when the maximum moves, up to 2^15.
+  constexpr float kUp = kBf ? 0.0f : 7.0f, kGrow = 8.0f;
+  constexpr int NS = L::kSlots, NR = L::kRawSlots;
+  constexpr uint32_t kTmemCols = 512;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t sbase = smem_u32(smem);
+  __shared__ uint64_t kv_full[kMaxSlots], kv_empty[kMaxSlots], raw_full[kMaxRaw], raw_empty[kMaxRaw], q_full, q_empty,
+      s_full[2], p_full[2], pv_done[2], joined, mma_done;
+  __shared__ uint32_t tmem_base_s;
+  __shared__ volatile int s_abort;
+  __shared__ PgShare share;
+  __shared__ int64_t scan[kThreads / 32];
+  __shared__ float join_s[2][kRows];             // [chain][row]: maxima, then sums, at the end of a deep item
+  __shared__ int8_t qexp_s[2][kE4m3 ? kTile : 1];   // e of a row's Q scale 2^-e, by item parity
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const PgTiles tiles{kTile, kKeys, a.group, kRows, 2 * kKeys};
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < NS; ++s) {
+      mbar_init(&kv_full[s], kE4m3 ? 4 : 1);
+      mbar_init(&kv_empty[s], 1);
+    }
+    for (int s = 0; s < NR; ++s) {
+      mbar_init(&raw_full[s], 1);
+      mbar_init(&raw_empty[s], 4);
+    }
+    mbar_init(&q_full, 4);
+    mbar_init(&q_empty, 1);
+    for (int c = 0; c < 2; ++c) {
+      mbar_init(&s_full[c], 1);
+      mbar_init(&p_full[c], 4);
+      mbar_init(&pv_done[c], 1);
+    }
+    mbar_init(&joined, 8);
+    mbar_init(&mma_done, 1);
+    s_abort = 0;
+    fence_mbar_init();
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&tk) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&tv) : "memory");
+  }
+  pdl_trigger();
+  pdl_wait();            // launched as a programmatic dependent: global data from here on
+  pg_share<kThreads>(a, tiles, blockIdx.x, gridDim.x, &share, scan, &g_tu_status);
+  if (threadIdx.x == 128) a.cut[blockIdx.x] = make_int4(-1, 0, 0, 0);      // (first thread of softmax group A)
+  if (share.left == 0) return;
+  const int D = a.D;
+
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_s)),
+                 "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_base_s;
+  PgWalk walk(share);
+  PgItem it;
+
+  if (warp == 0) {
+    // ---------------------------------------------------------------- TMA producer
+    // A tile is kKeys / box boxes of `box` keys, each inside one page; lane l serves box l % boxes.
+    const int boxes = kKeys / box;
+    const int bx = lane & (boxes - 1);
+    constexpr int NF = kE4m3 ? NR : NS;                        // ring the copies go to
+    uint64_t* const full = kE4m3 ? raw_full : kv_full;
+    uint64_t* const empty = kE4m3 ? raw_empty : kv_empty;
+    constexpr uint32_t kSlotBytes = kE4m3 ? L::kRaw : L::kOp;
+    const uint32_t bytes = kE4m3 ? (uint32_t)(kKeys * D) : kSlotBytes;
+    uint32_t u = 0;                                            // copies so far = tiles of the ring used
+    bool ok = true;
+    while (ok && walk.next(a, tiles, it)) {
+      const PcItem g(a, it);
+      const int32_t* bt = a.block_table + (int64_t)it.b * a.bt_stride;
+      auto page_of = [&](int kt, int& in) -> int {             // block and row of this lane's box of tile kt
+        const int key = kt * kKeys + bx * box;
+        in = 0;
+        if (key >= it.r.kl) return (int)a.num_blocks;          // past the last token: zeros
+        const int blk = key / a.bs;
+        in = key - blk * a.bs;
+        const int phys = __ldg(bt + blk);
+        if (phys < 0 || phys >= a.num_blocks) {
+          atomicOr(&g_tu_status, kStatusBadPage);
+          return (int)a.num_blocks;
+        }
+        return phys;
+      };
+      int in, phys = page_of(g.kt0, in);
+      for (int i = 0; i < g.T && ok; ++i) {
+        int in_next = 0, phys_next = 0;
+        if (i + 1 < g.T) phys_next = page_of(g.kt0 + i + 1, in_next);
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv, ++u) {
+          const uint32_t s = u % NF;
+          if (u >= NF && !warp_wait(&empty[s], ((u / NF) & 1) ^ 1)) s_abort = 1;
+          if (__any_sync(0xffffffffu, s_abort)) {
+            ok = false;
+            break;
+          }
+          if (lane == 0) mbar_arrive_expect_tx(&full[s], bytes);
+          __syncwarp();
+          const CUtensorMap* map = kv ? &tv : &tk;
+          if constexpr (kE4m3) {
+            const uint32_t pitch = ((uint32_t)(box * D) + 127u) & ~127u;
+            if (lane < boxes) tma_load_4d(sbase + L::kRaw0 + s * L::kRaw + bx * pitch, map, 0, it.h, in, phys, &full[s]);
+          } else {
+            for (int x = lane; x < DC * boxes; x += 32) {
+              const int c = x / boxes;
+              tma_load_4d(sbase + L::kKv0 + s * L::kOp + c * kChunkBytes + bx * box * 128, map, c * 64, it.h, in, phys,
+                          &full[s]);
+            }
+          }
+        }
+        phys = phys_next;
+        in = in_next;
+      }
+    }
+    // every copy this CTA issued has landed before it exits
+    for (uint32_t v = u > NF ? u - NF : 0; v < u; ++v) mbar_wait_bounded(&full[v % NF], (v / NF) & 1);
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------- MMA issuer (lane 0; the warp zeroes page tails)
+    constexpr uint32_t kIdS = idesc_f16(kRows, kKeys, kBf, false);
+    const uint32_t id_pv = idesc_f16(kRows, D, kBf, true);
+    const int ksteps = D / 16;
+    uint32_t u0 = 0, item = 0;                                 // ring position of the item's first tile
+    uint32_t ns[2] = {0, 0}, np[2] = {0, 0};                   // S and PV products of each chain so far
+    bool ok = true;
+    while (ok && walk.next(a, tiles, it)) {
+      const PcItem g(a, it);
+      const int n0 = g.count(0), n1 = g.count(1);
+      // S of chain c with the item's key tile i into the chain's S buffer; `last`: nothing else uses this K tile
+      auto issue_s = [&](int c, int i, bool last, bool last_s) -> bool {
+        const uint32_t v = u0 + 2 * i, s = v % NS;
+        if (!warp_wait(&kv_full[s], (v / NS) & 1)) return false;
+        if (ns[c] > 0 && !warp_wait(&pv_done[c], (ns[c] - 1) & 1)) return false;   // the P it overwrites is used up
+        tc_fence_after();
+        if (lane == 0) {
+          const uint32_t qb = sbase + L::kQ0 + (g.wide ? c : 0) * L::kOp, kb = sbase + L::kKv0 + s * L::kOp;
+          for (int ks = 0; ks < ksteps; ++ks) {
+            const uint32_t ob = (uint32_t)(ks >> 2) * kChunkBytes + (uint32_t)(ks & 3) * 32u;
+            mma_f16(tmem + (uint32_t)c * 256u, desc_kmajor(qb + ob), desc_kmajor(kb + ob), kIdS, ks > 0);
+          }
+          mma_commit(&s_full[c]);
+          if (last) mma_commit(&kv_empty[s]);
+          if (last_s) mma_commit(&q_empty);
+        }
+        ++ns[c];
+        return true;
+      };
+      auto issue_pv = [&](int c, int i, bool first, bool last) -> bool {
+        const uint32_t v = u0 + 2 * i + 1, s = v % NS;
+        if (!warp_wait(&kv_full[s], (v / NS) & 1)) return false;
+        if constexpr (!kE4m3) {
+          // rows of this V tile past the last token, up to the end of its box: whatever the page holds
+          const int end = it.r.kl - (g.kt0 + i) * kKeys;
+          if (end < kKeys && end > 0 && end % box && (!g.wide || c == 0 || g.TA <= i)) {
+            const int n = box - end % box;
+            for (int x = lane; x < n * 8 * DC; x += 32) {
+              const int r = end + x / (8 * DC), q = x % (8 * DC);
+              *reinterpret_cast<uint4*>(smem + L::kKv0 + s * L::kOp + (q >> 3) * kChunkBytes + r * 128 + (q & 7) * 16) =
+                  make_uint4(0u, 0u, 0u, 0u);
+            }
+            fence_async_smem();
+            __syncwarp();
+          }
+        }
+        if (!warp_wait(&p_full[c], np[c] & 1)) return false;
+        tc_fence_after();
+        if (lane == 0) {
+          const uint32_t vb = sbase + L::kKv0 + s * L::kOp;
+          const uint32_t tb = tmem + (uint32_t)c * 256u;
+#pragma unroll
+          for (int ks = 0; ks < kKeys / 16; ++ks)   // P: 16 keys = 8 packed columns over the scores
+            mma_f16_ts(tb + 128u, tb + (uint32_t)ks * 8u, desc_mnmajor(vb + (uint32_t)ks * 2048u, kChunkBytes), id_pv,
+                       !first || ks > 0);
+          mma_commit(&pv_done[c]);
+          if (last) mma_commit(&kv_empty[s]);
+        }
+        ++np[c];
+        return true;
+      };
+      ok = warp_wait(&q_full, item & 1);
+      ++item;
+      if (g.wide) {
+        if (ok && n0 > 0) ok = issue_s(0, 0, false, false);
+        if (ok) ok = issue_s(1, 0, true, g.T == 1);
+        for (int i = 0; i < g.T && ok; ++i) {
+          if (i < n0) {
+            ok = issue_pv(0, i, i == 0, false);
+            if (ok && i + 1 < n0) ok = issue_s(0, i + 1, false, false);
+          }
+          if (ok) ok = issue_pv(1, i, i == 0, true);
+          if (ok && i + 1 < g.T) ok = issue_s(1, i + 1, true, i + 2 == g.T);
+        }
+      } else {
+        ok = ok && issue_s(0, 0, true, g.T == 1);
+        if (ok && n1 > 0) ok = issue_s(1, 1, true, g.T == 2);
+        for (int i = 0; i < g.T && ok; ++i) {
+          ok = issue_pv(i & 1, i, i < 2, true);
+          if (ok && i + 2 < g.T) ok = issue_s(i & 1, i + 2, true, i + 3 == g.T);
+        }
+      }
+      u0 += 2 * g.T;
+      ok = __all_sync(0xffffffffu, ok && !s_abort);
+    }
+    if (!ok) s_abort = 1;
+    if (lane == 0) {
+      mma_commit(&mma_done);                 // every MMA issued above has completed before TMEM is freed
+      mbar_wait_bounded(&mma_done, 0);
+    }
+  } else if (warp < 4 || warp >= 12) {
+    // ---------------------------------------------------------------- helpers: query rows, e4m3 codes to float16
+    const int ht = (warp < 4 ? warp - 2 : warp - 10) * 32 + lane;          // 0 .. 127
+    uint32_t u = 0, item = 0;
+    bool ok = true;
+    while (ok && walk.next(a, tiles, it)) {
+      const PcItem g(a, it);
+      if (item > 0 && !warp_wait(&q_empty, (item - 1) & 1)) s_abort = 1;
+      if (__any_sync(0xffffffffu, s_abort)) break;
+      {
+        // Sixteen lanes (eight for D <= 64) take a row: eight elements each, whole rows coalesced.
+        constexpr int LPR = 8 * DC;
+        const int nrows = g.wide ? kTile : kRows;
+        const int q8 = ht % LPR;
+        const T* qg = reinterpret_cast<const T*>(a.q) + (int64_t)it.r.q0 * a.q_ts + (int64_t)it.h * a.group * D + q8 * 8;
+        const uint32_t dst0 = sbase + L::kQ0 + (q8 >> 3) * kChunkBytes;
+        constexpr int RPI = kHelpers / LPR;                                 // rows per pass
+        if constexpr (!kE4m3) {
+          for (int r = ht / LPR; r < nrows; r += RPI) {
+            const int gr = g.row0 + r;
+            const bool in = r < g.rows && q8 * 8 < D;
+            const int tok = in ? gr / a.group : 0;
+            const T* src = in ? qg + (int64_t)tok * a.q_ts + (gr - tok * a.group) * D
+                              : reinterpret_cast<const T*>(a.q);
+            const uint32_t dst = dst0 + (r >> 7) * L::kOp + (r & 127) * 128 + (((q8 & 7) ^ (r & 7)) << 4);
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+          }
+          asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+        } else {
+          constexpr int U = 4;                                              // rows in flight per thread
+          for (int rb = ht / LPR; rb < nrows; rb += U * RPI) {
+            Vec8<T> x[U];
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+              const int r = rb + i * RPI, gr = g.row0 + r;
+              x[i].w[0] = make_uint4(0u, 0u, 0u, 0u);
+              if (r < g.rows && q8 * 8 < D) {
+                const int tok = gr / a.group;
+                x[i].load(qg + (int64_t)tok * a.q_ts + (gr - tok * a.group) * D);
+              }
+            }
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+              const int r = rb + i * RPI;
+              float f[8];
+              x[i].unpack(f);
+              float mx = 0.0f;
+#pragma unroll
+              for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(f[e]));
+#pragma unroll
+              for (int o = LPR / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+              // e: the exponent of the row's largest element, within what 2^e and 2^-e have
+              const int e2 = min(max((int)(__float_as_uint(mx) >> 23) - 127, -100), 120);
+              const float up = __int_as_float((127 - e2) << 23);
+              Vec8<__half> h;
+#pragma unroll
+              for (int e = 0; e < 8; ++e) f[e] *= up;
+              h.pack(f);
+              *reinterpret_cast<uint4*>(smem + (dst0 - sbase) + (r >> 7) * L::kOp + (r & 127) * 128 +
+                                        (((q8 & 7) ^ (r & 7)) << 4)) = h.w[0];
+              if (q8 == 0) qexp_s[item & 1][r] = (int8_t)e2;
+            }
+          }
+        }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&q_full);
+        ++item;
+      }
+      if constexpr (kE4m3) {
+        const uint32_t pitch = ((uint32_t)(box * D) + 127u) & ~127u;
+        const int chunks = D / 16;                              // 16 codes a chunk
+        for (int i = 0; i < 2 * g.T && ok; ++i, ++u) {
+          const uint32_t sr = u % NR, s = u % NS;
+          if (!warp_wait(&raw_full[sr], (u / NR) & 1)) s_abort = 1;
+          if (u >= NS && !warp_wait(&kv_empty[s], ((u / NS) & 1) ^ 1)) s_abort = 1;
+          if (__any_sync(0xffffffffu, s_abort)) {
+            ok = false;
+            break;
+          }
+          const uint8_t* raw = smem + L::kRaw0 + sr * L::kRaw;
+          uint8_t* dst = smem + L::kKv0 + s * L::kOp;
+          const int end = it.r.kl - (g.kt0 + (i >> 1)) * kKeys;  // rows from here on are past the last token
+          // thread: chunk ht % (4 DC) of rows ht / (4 DC), + 128 / (4 DC), ...
+          constexpr int CPR = 4 * DC;
+          const int c = ht % CPR;
+          if (c < chunks) {
+#pragma unroll 4
+            for (int r = ht / CPR; r < kKeys; r += kHelpers / CPR) {
+              uint4 x = *reinterpret_cast<const uint4*>(raw + (r / box) * pitch + (r % box) * D + c * 16);
+              if (r >= end) x = make_uint4(0u, 0u, 0u, 0u);
+              const uint4 lo = make_uint4(e4m3x2_to_f16x2(x.x), e4m3x2_to_f16x2(x.x >> 16), e4m3x2_to_f16x2(x.y),
+                                          e4m3x2_to_f16x2(x.y >> 16));
+              const uint4 hi = make_uint4(e4m3x2_to_f16x2(x.z), e4m3x2_to_f16x2(x.z >> 16), e4m3x2_to_f16x2(x.w),
+                                          e4m3x2_to_f16x2(x.w >> 16));
+              uint8_t* d = dst + (c >> 2) * kChunkBytes + r * 128;
+              const int q = (2 * c) & 7;
+              *reinterpret_cast<uint4*>(d + ((q ^ (r & 7)) << 4)) = lo;
+              *reinterpret_cast<uint4*>(d + (((q + 1) ^ (r & 7)) << 4)) = hi;
+            }
+          }
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&kv_full[s]);
+            mbar_arrive(&raw_empty[sr]);
+          }
+        }
+      }
+    }
+  } else {
+    // ---------------------------------------------------------------- softmax (warps 4-7: chain A, 8-11: chain B)
+    const int c = (warp - 4) >> 2;
+    const int quarter = warp & 3;                          // TMEM lanes this warp may access
+    const int row = quarter * 32 + lane;                   // row of the chain = TMEM lane
+    const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
+    const uint32_t s_col = tmem + lane_addr + (uint32_t)c * 256u, o_col = s_col + 128u;
+    uint32_t n = 0, item = 0;                              // tiles of the chain so far; items
+    int64_t at = walk.at;                                  // first unit of the item's part
+    uint32_t joins = 0;
+    bool ok = true;
+    auto join = [&]() -> bool {                            // a barrier of the two groups, bounded like every wait
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&joined);
+      const bool met = warp_wait(&joined, joins & 1);
+      ++joins;
+      tc_fence_after();
+      return met;
+    };
+    while (ok && walk.next(a, tiles, it)) {
+      const PcItem g(a, it);
+      const int trow = (g.wide ? c * kRows : 0) + row;     // row of the tile
+      const bool valid = trow < g.rows;
+      const bool any_valid = (g.wide ? c * kRows : 0) + quarter * 32 < g.rows;
+      const int gr = g.row0 + trow;
+      const int off = it.r.kl - it.r.ql;
+      const int tok = valid ? gr / a.group : 0;
+      const int pos = valid ? off + tok : it.r.kl - 1;     // rows past the request compute on zeros, unseen
+      const int pos_min = off + (g.row0 + (g.wide ? c * kRows : 0) + quarter * 32) / a.group;
+      float sc = a.scale_log2;
+      const int nt = g.count(c);
+      if constexpr (kE4m3) {
+        if (nt > 0) {
+          if (!warp_wait(&q_full, item & 1)) s_abort = 1;
+          sc *= __ldg(a.k_scale + it.h) * __int_as_float((127 + (int)qexp_s[item & 1][trow]) << 23);
+        }
+      }
+      if (sc == 0.0f) sc = 1e-30f;                         // equal weights; a masked score stays -inf below
+      const float hidden = sc >= 0.0f ? -INFINITY : INFINITY;
+      float m = -INFINITY, l = 0.0f;
+      for (int i = 0; i < nt; ++i, ++n) {
+        if (__shfl_sync(0xffffffffu, s_abort, 0) || !warp_wait(&s_full[c], n & 1)) {   // warp-uniform
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        if (any_valid) {
+          const int kb = (g.kt0 + (g.wide ? i : 2 * i + c)) * kKeys;
+          const bool mask = kb + kKeys - 1 > pos_min;      // some key of the tile may pass a row
+          // The maximum over the upper 64 scores, then over the lower 64, which stay in registers: P of the
+          // lower half goes over columns that have been read, then the upper half is loaded once more.
+          uint32_t r[64];
+          float mx4[4];
+          const float none = sc >= 0.0f ? -INFINITY : INFINITY;
+          mx4[0] = mx4[1] = mx4[2] = mx4[3] = none;
+#pragma unroll
+          for (int hf = 1; hf >= 0; --hf) {
+            tmem_ld64_async(s_col + 64u * hf, r);
+            tmem_ld_wait(r);
+            if (mask) {
+#pragma unroll
+              for (int e = 0; e < 64; ++e)
+                if (kb + 64 * hf + e > pos) r[e] = __float_as_uint(hidden);
+            }
+            if (sc >= 0.0f) {
+#pragma unroll
+              for (int e = 0; e < 64; ++e) mx4[e & 3] = fmaxf(mx4[e & 3], __uint_as_float(r[e]));
+            } else {
+#pragma unroll
+              for (int e = 0; e < 64; ++e) mx4[e & 3] = fminf(mx4[e & 3], __uint_as_float(r[e]));
+            }
+          }
+          const float ext = sc >= 0.0f ? fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]))
+                                       : fminf(fminf(mx4[0], mx4[1]), fminf(mx4[2], mx4[3]));
+          const float mx = ext * sc - kUp;                 // log2 domain; -inf where the row sees nothing
+          const bool grow = mx > m + kGrow;
+          const float alpha = grow ? ex2_approx(m - mx) : 1.0f;
+          if (grow) m = mx;
+          l *= alpha;
+          const float neg_m = m == -INFINITY ? 0.0f : -m;
+          float l4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {
+            if (hf == 1) {
+              tmem_ld64_async(s_col + 64u, r);
+              tmem_ld_wait(r);
+              if (mask) {
+#pragma unroll
+                for (int e = 0; e < 64; ++e)
+                  if (kb + 64 + e > pos) r[e] = __float_as_uint(hidden);
+              }
+            }
+            uint32_t w[32];
+#pragma unroll
+            for (int e = 0; e < 64; e += 2) {
+              const float p0 = ex2_approx(fmaf(__uint_as_float(r[e]), sc, neg_m));
+              const float p1 = ex2_approx(fmaf(__uint_as_float(r[e + 1]), sc, neg_m));
+              l4[(e >> 1) & 3] += p0 + p1;
+              w[e >> 1] = pack2h<kBf>(p0, p1);
+            }
+            tmem_st32(s_col + 32u * hf, w);
+          }
+          l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
+          // O *= alpha where the maximum moved (the whole warp, when any of its rows needs it), once the
+          // chain's last PV has completed
+          if (i > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
+            if (!warp_wait(&pv_done[c], (n - 1) & 1)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            for (int x = 0; x < (D + 31) / 32; ++x) {
+              uint32_t o[32];
+              tmem_ld32(o_col + x * 32, o);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+              tmem_st32(o_col + x * 32, o);
+            }
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[c]);
+      }
+      if (ok && nt > 0) ok = warp_wait(&pv_done[c], (n - 1) & 1);
+      tc_fence_after();
+      if (!ok) s_abort = 1;
+      // ---- the item's result: finished, or a part of it
+      float w_own = 1.0f, w_other = 0.0f;
+      bool has_other = false;
+      if (!g.wide) {
+        // exchange through one array: maxima, then (once they have been read) sums
+        join_s[c][row] = m;
+        ok = join() && ok;
+        const float m2 = join_s[c ^ 1][row];
+        ok = join() && ok;
+        join_s[c][row] = l;
+        ok = join() && ok;
+        const float l2 = join_s[c ^ 1][row];
+        const float mj = fmaxf(m, m2), mu = mj == -INFINITY ? 0.0f : mj;
+        w_own = ex2_approx(m - mu);
+        w_other = ex2_approx(m2 - mu);
+        l = l * w_own + l2 * w_other;
+        m = mj;
+        has_other = g.count(c ^ 1) > 0;
+      }
+      if (ok && any_valid) {
+        const float vsc = kE4m3 ? __ldg(a.v_scale + it.h) : 1.0f;
+        const bool whole = it.whole();
+        const float fin = whole ? (l > 0.0f ? vsc / l : 0.0f) : vsc;
+        const int64_t slot = 2 * (int64_t)blockIdx.x + (it.j0 == 0 ? 1 : 0);
+        const int64_t orow = (int64_t)(it.r.q0 + tok) * a.hq + it.h * a.group + (gr - tok * a.group);
+        T* og = reinterpret_cast<T*>(a.out) + orow * D;
+        float* po = a.part_o + (slot * kTile + trow) * D;
+        if (valid && (g.wide || c == 0)) {
+          if (whole) {
+            if (a.lse) a.lse[orow] = (m + log2f(l)) * kPgLn2;
+          } else {
+            float* ml = a.part_ml + slot * 2 * kTile;
+            ml[trow] = m;
+            ml[kTile + trow] = l;
+          }
+        }
+        // sixteen columns at a time; in a deep item chain A stores the even sixteens and B the odd ones
+        for (int x = g.wide ? 0 : c; x < D / 16; x += g.wide ? 1 : 2) {
+          uint32_t o[16], o2[16];
+          float f[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[e] = o2[e] = 0u;
+          if (nt > 0) tmem_ld16_async(o_col + x * 16, o);
+          if (has_other) tmem_ld16_async((o_col ^ 256u) + x * 16, o2);
+          tmem_ld_wait(o);
+          tmem_ld_wait(o2);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            float y = __uint_as_float(o[e]);
+            if (!g.wide) y = y * w_own + __uint_as_float(o2[e]) * w_other;
+            f[e] = y * fin;
+          }
+          if (!valid) continue;
+          if (whole) {
+            uint32_t w[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e] = pack2h<std::is_same<T, __nv_bfloat16>::value>(f[2 * e], f[2 * e + 1]);
+            *reinterpret_cast<uint4*>(og + x * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+            *reinterpret_cast<uint4*>(og + x * 16 + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              *reinterpret_cast<float4*>(po + x * 16 + 4 * e) = make_float4(f[4 * e], f[4 * e + 1], f[4 * e + 2], f[4 * e + 3]);
+          }
+        }
+      }
+      if (!it.whole() && it.j0 == 0 && threadIdx.x == 128)
+        a.cut[blockIdx.x] = make_int4(g.row0, it.b, it.h, pg_cta_of(at + it.n - 1, share.total, share.ctas));
+      if (!g.wide) ok = join() && ok;                      // both groups have read both O before either moves on
+      if (!ok) s_abort = 1;
+      at += it.j1 - it.j0;
+      ++item;
+    }
+    if (!ok) s_abort = 1;
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+  }
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_tiled() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    cudaDriverEntryPointQueryResult q;
+    void* p = nullptr;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  });
+  return fn;
+}
+
+// [blocks, bs, hkv, D] cache: boxes of `box` keys of one page and one head; 16-bit elements 64 at a time
+// with the 128-byte swizzle, codes whole rows at a time.
+int make_page_map(CUtensorMap* map, const void* base, bool e4m3, bool bf16, const PagedArgs& a, int64_t block_stride, int box) {
+  auto fn = encode_tiled();
+  if (!fn) return set_error(KVB_E_LAUNCH, "paged_prefill_attention: cuTensorMapEncodeTiled unavailable");
+  const cuuint64_t es = e4m3 ? 1 : 2;
+  cuuint64_t dims[4] = {(cuuint64_t)a.D, (cuuint64_t)a.hkv, (cuuint64_t)a.bs, (cuuint64_t)a.num_blocks};
+  cuuint64_t strides[3] = {(cuuint64_t)a.D * es, (cuuint64_t)a.hkv * a.D * es, (cuuint64_t)block_stride * es};
+  cuuint32_t boxes[4] = {e4m3 ? (cuuint32_t)a.D : 64u, 1u, (cuuint32_t)box, 1u};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = fn(map, e4m3 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                  4, const_cast<void*>(base), dims, strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  e4m3 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(KVB_E_LAUNCH, "paged_prefill_attention: tensor map failed (%d)", (int)r);
+  return KVB_OK;
+}
+
+template <typename T, bool kE4m3, int DC>
+int launch_pc(const CUtensorMap& mk, const CUtensorMap& mv, const PagedArgs& a, int box, int grid, cudaStream_t st) {
+  constexpr size_t smem = PcLayout<kE4m3, DC>::kSmem;
+  auto kern = paged_prefill_tc_kernel<T, kE4m3, DC>;
+  // every call: the attribute belongs to the current device's copy of the kernel
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e == cudaSuccess) e = launch_pdl(kern, dim3((unsigned)grid), dim3(kThreads), smem, st, mk, mv, a, box);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return set_error(KVB_E_LAUNCH, "paged_prefill_tc_kernel: %s", cudaGetErrorString(e));
+  }
+  return check_launch("paged_prefill_tc_kernel");
+}
+
+}  // namespace
+
+// Whether the tcgen05 kernel takes the case: 16-bit queries, head_dim a multiple of 16 in [64, 128], and
+// pages that a tile of 128 keys is cut into at most 32 boxes by (a box lies in one page, its rows start on
+// the 128-byte grid that TMA wants).
+bool paged_prefill_tc_takes(const PagedArgs& a, int q_dtype, int cache_dtype) {
+  const int cs = cache_dtype == KVB_E4M3 ? 1 : 2;
+  return (q_dtype == KVB_BF16 || q_dtype == KVB_F16) && a.D % 16 == 0 && a.D >= 64 && a.D <= 128 && a.bs % 4 == 0 &&
+         aligned16(a.k_cache) && aligned16(a.v_cache) && (a.k_bs * cs) % 16 == 0 && (a.v_bs * cs) % 16 == 0 &&
+         a.num_blocks > 0 && a.num_blocks < INT32_MAX;
+}
+
+int paged_prefill_tcgen05(PagedArgs& a, int q_dtype, int cache_dtype, void* ws, int sms, cudaStream_t st) {
+  int box = kKeys;
+  while (a.bs % box) box >>= 1;
+  const bool e4 = cache_dtype == KVB_E4M3, bf = q_dtype == KVB_BF16;
+  CUtensorMap mk, mv;
+  int rc = make_page_map(&mk, a.k_cache, e4, bf, a, a.k_bs, box);
+  if (!rc) rc = make_page_map(&mv, a.v_cache, e4, bf, a, a.v_bs, box);
+  if (rc) return rc;
+  pg_workspace_layout(a, ws, sms, kTile);
+  using B = __nv_bfloat16;
+  using H = __half;
+  if (a.D <= 64) {
+    if (bf) rc = e4 ? launch_pc<B, true, 1>(mk, mv, a, box, sms, st) : launch_pc<B, false, 1>(mk, mv, a, box, sms, st);
+    else rc = e4 ? launch_pc<H, true, 1>(mk, mv, a, box, sms, st) : launch_pc<H, false, 1>(mk, mv, a, box, sms, st);
+  } else {
+    if (bf) rc = e4 ? launch_pc<B, true, 2>(mk, mv, a, box, sms, st) : launch_pc<B, false, 2>(mk, mv, a, box, sms, st);
+    else rc = e4 ? launch_pc<H, true, 2>(mk, mv, a, box, sms, st) : launch_pc<H, false, 2>(mk, mv, a, box, sms, st);
+  }
+  if (rc) return rc;
+  return pg_launch_merge(a, q_dtype, kTile, sms, st);
+}
+
+}  // namespace kvb
