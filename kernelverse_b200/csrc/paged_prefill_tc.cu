@@ -11,9 +11,12 @@
 //     use every K/V tile of 128 keys;
 //   deep items (at most 128 rows: decoding, drafts, the last rows of a prompt): both chains have the
 //     same rows, A takes the even K/V tiles and B the odd ones, and the two results are joined.
-// Roles: warp 0 issues the TMA loads (boxes of whole page runs gathered through the block table);
-// warp 1 owns TMEM and issues the MMAs; warps 2, 3, 12, 13 gather the query rows and turn e4m3 codes
-// into float16 operands; warps 4-7 and 8-11 are the softmax groups of A and B.
+// Roles: warp 0 issues the TMA loads (boxes of whole page runs gathered through the block table); one
+// lane each of warps 1 and 2 issues the MMAs of chain A and of chain B (one issuer for both was the
+// limit: its 16 MMAs, four commits and four waits a tile took ~2900 cycles, against 1024 of tensor
+// time); warp 3 zeroes page tails; warps 4-7 and 8-11 are the softmax groups of A and B; warps 12-15
+// gather the query rows and turn e4m3 codes into float16 operands.  The softmax warps take the
+// registers that the others give up (a row's 128 scores stay in registers).
 // K and V tiles share one ring of shared-memory slots in the order K_0 V_0 K_1 V_1 ...  A page outside
 // the cache, and pages past the last token, are loaded from an out-of-range block coordinate, which
 // TMA fills with zeros; the rows past the last token inside its page are zeroed in shared memory.
@@ -38,8 +41,9 @@ namespace {
 constexpr int kRows = 128;                 // rows of a chain (TMEM lanes)
 constexpr int kKeys = 128;                 // keys per K/V tile
 constexpr int kTile = 2 * kRows;           // rows of a tile
-constexpr int kThreads = 448;
-constexpr int kHelpers = 128;              // threads of warps 2, 3, 12, 13
+constexpr int kThreads = 512;
+constexpr int kHelpers = 128;              // threads of warps 12-15
+constexpr int kSoftmaxRegs = 192, kOtherRegs = 64;   // 2 x 128 x (192 + 64) = 512 x 128: what the block is launched with
 constexpr int kMaxSlots = 8;
 constexpr int kMaxRaw = 4;
 
@@ -99,7 +103,27 @@ struct PcItem {
   }
   // tiles of chain c, the first one and the step to the next
   __device__ __forceinline__ int count(int c) const { return wide ? (c ? T : TA) : (T - c + 1) >> 1; }
+  // whether one chain alone uses the item's tile i
+  __device__ __forceinline__ bool one_user(int i) const { return !wide || i >= TA; }
 };
+// Rows of key tile kt past the last token that a box of the tile holds together with tokens.
+__device__ __forceinline__ int tail_rows(int kl, int kt, int box) {
+  const int end = kl - kt * kKeys, in = end & (box - 1);
+  return end > 0 && end < kKeys && in ? box - in : 0;
+}
+
+template <int N> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float min3(float a, float b, float c) {
+  float r;
+  asm("min.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 
 template <typename T, bool kE4m3, int DC>
 __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __grid_constant__ CUtensorMap tk,
@@ -114,8 +138,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_u32(smem);
-  __shared__ uint64_t kv_full[kMaxSlots], kv_empty[kMaxSlots], raw_full[kMaxRaw], raw_empty[kMaxRaw], q_full, q_empty,
-      s_full[2], p_full[2], pv_done[2], joined, mma_done;
+  __shared__ uint64_t kv_full[kMaxSlots], kv_empty[kMaxSlots], tail_full[kE4m3 ? 1 : kMaxSlots],
+      raw_full[kE4m3 ? kMaxRaw : 1], raw_empty[kE4m3 ? kMaxRaw : 1],
+      q_full, q_empty, s_full[2], p_full[2], pv_done[2], mma_done[2], joined;
   __shared__ uint32_t tmem_base_s;
   __shared__ volatile int s_abort;
   __shared__ PgShare share;
@@ -128,21 +153,22 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
   if (threadIdx.x == 0) {
     for (int s = 0; s < NS; ++s) {
       mbar_init(&kv_full[s], kE4m3 ? 4 : 1);
-      mbar_init(&kv_empty[s], 1);
+      mbar_init(&kv_empty[s], 2);            // one arrival for each chain
+      if constexpr (!kE4m3) mbar_init(&tail_full[s], 1);
     }
     for (int s = 0; s < NR; ++s) {
       mbar_init(&raw_full[s], 1);
       mbar_init(&raw_empty[s], 4);
     }
     mbar_init(&q_full, 4);
-    mbar_init(&q_empty, 1);
+    mbar_init(&q_empty, 2);
     for (int c = 0; c < 2; ++c) {
       mbar_init(&s_full[c], 1);
       mbar_init(&p_full[c], 4);
       mbar_init(&pv_done[c], 1);
+      mbar_init(&mma_done[c], 1);
     }
     mbar_init(&joined, 8);
-    mbar_init(&mma_done, 1);
     s_abort = 0;
     fence_mbar_init();
     asm volatile("prefetch.tensormap [%0];" ::"l"(&tk) : "memory");
@@ -168,10 +194,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
   PgWalk walk(share);
   PgItem it;
 
+  if (warp < 4) {
+  regs_down<kOtherRegs>();
   if (warp == 0) {
     // ---------------------------------------------------------------- TMA producer
     // A tile is kKeys / box boxes of `box` keys, each inside one page; lane l serves box l % boxes.
-    const int boxes = kKeys / box;
+    const int boxes = kKeys / box, lboxes = __ffs(boxes) - 1;
     const int bx = lane & (boxes - 1);
     constexpr int NF = kE4m3 ? NR : NS;                        // ring the copies go to
     uint64_t* const full = kE4m3 ? raw_full : kv_full;
@@ -208,17 +236,23 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
             ok = false;
             break;
           }
-          if (lane == 0) mbar_arrive_expect_tx(&full[s], bytes);
-          __syncwarp();
           const CUtensorMap* map = kv ? &tv : &tk;
+          uint64_t* bar = &full[s];
+          if constexpr (!kE4m3) {
+            // a V tile whose last page has rows past the last token goes through warp 3
+            if (kv && tail_rows(it.r.kl, g.kt0 + i, box) > 0) bar = &tail_full[s];
+            // the slot's release takes an arrival of each chain: this one stands for a chain that does not use the tile
+            if (lane == 0 && g.one_user(i)) mbar_arrive(&empty[s]);
+          }
+          if (lane == 0) mbar_arrive_expect_tx(bar, bytes);
+          __syncwarp();
           if constexpr (kE4m3) {
             const uint32_t pitch = ((uint32_t)(box * D) + 127u) & ~127u;
-            if (lane < boxes) tma_load_4d(sbase + L::kRaw0 + s * L::kRaw + bx * pitch, map, 0, it.h, in, phys, &full[s]);
+            if (lane < boxes) tma_load_4d(sbase + L::kRaw0 + s * L::kRaw + bx * pitch, map, 0, it.h, in, phys, bar);
           } else {
             for (int x = lane; x < DC * boxes; x += 32) {
-              const int c = x / boxes;
-              tma_load_4d(sbase + L::kKv0 + s * L::kOp + c * kChunkBytes + bx * box * 128, map, c * 64, it.h, in, phys,
-                          &full[s]);
+              const int c = x >> lboxes;
+              tma_load_4d(sbase + L::kKv0 + s * L::kOp + c * kChunkBytes + bx * box * 128, map, c * 64, it.h, in, phys, bar);
             }
           }
         }
@@ -226,102 +260,104 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
         in = in_next;
       }
     }
-    // every copy this CTA issued has landed before it exits
+    // every copy this CTA issued has landed before it exits (tails: warp 3 has seen theirs)
     for (uint32_t v = u > NF ? u - NF : 0; v < u; ++v) mbar_wait_bounded(&full[v % NF], (v / NF) & 1);
-  } else if (warp == 1) {
-    // ---------------------------------------------------------------- MMA issuer (lane 0; the warp zeroes page tails)
-    constexpr uint32_t kIdS = idesc_f16(kRows, kKeys, kBf, false);
-    const uint32_t id_pv = idesc_f16(kRows, D, kBf, true);
-    const int ksteps = D / 16;
-    uint32_t u0 = 0, item = 0;                                 // ring position of the item's first tile
-    uint32_t ns[2] = {0, 0}, np[2] = {0, 0};                   // S and PV products of each chain so far
-    bool ok = true;
-    while (ok && walk.next(a, tiles, it)) {
-      const PcItem g(a, it);
-      const int n0 = g.count(0), n1 = g.count(1);
-      // S of chain c with the item's key tile i into the chain's S buffer; `last`: nothing else uses this K tile
-      auto issue_s = [&](int c, int i, bool last, bool last_s) -> bool {
-        const uint32_t v = u0 + 2 * i, s = v % NS;
-        if (!warp_wait(&kv_full[s], (v / NS) & 1)) return false;
-        if (ns[c] > 0 && !warp_wait(&pv_done[c], (ns[c] - 1) & 1)) return false;   // the P it overwrites is used up
-        tc_fence_after();
-        if (lane == 0) {
-          const uint32_t qb = sbase + L::kQ0 + (g.wide ? c : 0) * L::kOp, kb = sbase + L::kKv0 + s * L::kOp;
-          for (int ks = 0; ks < ksteps; ++ks) {
-            const uint32_t ob = (uint32_t)(ks >> 2) * kChunkBytes + (uint32_t)(ks & 3) * 32u;
-            mma_f16(tmem + (uint32_t)c * 256u, desc_kmajor(qb + ob), desc_kmajor(kb + ob), kIdS, ks > 0);
+  } else if (warp <= 2) {
+    // ---------------------------------------------------------------- MMA issuers: lane 0 of warp 1 + c, chain c
+    if (lane == 0) {
+      const int c = warp - 1;
+      const uint32_t tb = tmem + (uint32_t)c * 256u;
+      constexpr uint32_t kIdS = idesc_f16(kRows, kKeys, kBf, false);
+      const uint32_t id_pv = idesc_f16(kRows, D, kBf, true);
+      uint32_t u0 = 0, item = 0;                               // ring position of the item's first tile
+      uint32_t n = 0;                                          // tiles of the chain whose S has been issued
+      bool ok = true;
+      while (ok && walk.next(a, tiles, it)) {
+        const PcItem g(a, it);
+        const int count = g.count(c), first = g.wide ? 0 : c, step = g.wide ? 1 : 2;
+        const uint64_t qd = desc_kmajor(sbase + L::kQ0 + (g.wide ? c : 0) * L::kOp);
+        // S of the chain's tile k: item tile first + k * step
+        auto issue_s = [&](int k) -> bool {
+          const uint32_t v = u0 + 2 * (first + k * step), s = v % NS;
+          if (!mbar_wait_bounded(&kv_full[s], (v / NS) & 1)) return false;
+          if (n > 0 && !mbar_wait_bounded(&pv_done[c], (n - 1) & 1)) return false;   // the P it overwrites is used up
+          tc_fence_after();
+          const uint64_t kd = desc_kmajor(sbase + L::kKv0 + s * L::kOp);
+          // 16 elements = 32 bytes on in both operands, 64 elements one chunk on
+          if (D == 64 * DC) {
+#pragma unroll
+            for (int ks = 0; ks < 4 * DC; ++ks)
+              mma_f16(tb, qd + (ks >> 2) * (kChunkBytes >> 4) + (ks & 3) * 2, kd + (ks >> 2) * (kChunkBytes >> 4) + (ks & 3) * 2,
+                      kIdS, ks > 0);
+          } else {
+            for (int ks = 0; ks < D / 16; ++ks)
+              mma_f16(tb, qd + (ks >> 2) * (kChunkBytes >> 4) + (ks & 3) * 2, kd + (ks >> 2) * (kChunkBytes >> 4) + (ks & 3) * 2,
+                      kIdS, ks > 0);
           }
           mma_commit(&s_full[c]);
-          if (last) mma_commit(&kv_empty[s]);
-          if (last_s) mma_commit(&q_empty);
-        }
-        ++ns[c];
-        return true;
-      };
-      auto issue_pv = [&](int c, int i, bool first, bool last) -> bool {
-        const uint32_t v = u0 + 2 * i + 1, s = v % NS;
-        if (!warp_wait(&kv_full[s], (v / NS) & 1)) return false;
-        if constexpr (!kE4m3) {
-          // rows of this V tile past the last token, up to the end of its box: whatever the page holds
-          const int end = it.r.kl - (g.kt0 + i) * kKeys;
-          if (end < kKeys && end > 0 && end % box && (!g.wide || c == 0 || g.TA <= i)) {
-            const int n = box - end % box;
-            for (int x = lane; x < n * 8 * DC; x += 32) {
-              const int r = end + x / (8 * DC), q = x % (8 * DC);
-              *reinterpret_cast<uint4*>(smem + L::kKv0 + s * L::kOp + (q >> 3) * kChunkBytes + r * 128 + (q & 7) * 16) =
-                  make_uint4(0u, 0u, 0u, 0u);
-            }
-            fence_async_smem();
-            __syncwarp();
-          }
-        }
-        if (!warp_wait(&p_full[c], np[c] & 1)) return false;
-        tc_fence_after();
-        if (lane == 0) {
-          const uint32_t vb = sbase + L::kKv0 + s * L::kOp;
-          const uint32_t tb = tmem + (uint32_t)c * 256u;
+          mma_commit(&kv_empty[s]);
+          if (k + 1 == count) mma_commit(&q_empty);
+          ++n;
+          return true;
+        };
+        ok = mbar_wait_bounded(&q_full, item & 1);
+        ++item;
+        if (count == 0 && ok) mbar_arrive(&q_empty);
+        if (count > 0) ok = ok && issue_s(0);
+        for (int k = 0; k < count && ok; ++k) {
+          const uint32_t v = u0 + 2 * (first + k * step) + 1, s = v % NS;
+          ok = mbar_wait_bounded(&kv_full[s], (v / NS) & 1) && mbar_wait_bounded(&p_full[c], (n - 1) & 1);
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t vd = desc_mnmajor(sbase + L::kKv0 + s * L::kOp, kChunkBytes);
 #pragma unroll
           for (int ks = 0; ks < kKeys / 16; ++ks)   // P: 16 keys = 8 packed columns over the scores
-            mma_f16_ts(tb + 128u, tb + (uint32_t)ks * 8u, desc_mnmajor(vb + (uint32_t)ks * 2048u, kChunkBytes), id_pv,
-                       !first || ks > 0);
+            mma_f16_ts(tb + 128u, tb + (uint32_t)ks * 8u, vd + ks * 128, id_pv, (k | ks) != 0);
           mma_commit(&pv_done[c]);
-          if (last) mma_commit(&kv_empty[s]);
+          mma_commit(&kv_empty[s]);
+          if (k + 1 < count) ok = issue_s(k + 1);
         }
-        ++np[c];
-        return true;
-      };
-      ok = warp_wait(&q_full, item & 1);
-      ++item;
-      if (g.wide) {
-        if (ok && n0 > 0) ok = issue_s(0, 0, false, false);
-        if (ok) ok = issue_s(1, 0, true, g.T == 1);
-        for (int i = 0; i < g.T && ok; ++i) {
-          if (i < n0) {
-            ok = issue_pv(0, i, i == 0, false);
-            if (ok && i + 1 < n0) ok = issue_s(0, i + 1, false, false);
-          }
-          if (ok) ok = issue_pv(1, i, i == 0, true);
-          if (ok && i + 1 < g.T) ok = issue_s(1, i + 1, true, i + 2 == g.T);
-        }
-      } else {
-        ok = ok && issue_s(0, 0, true, g.T == 1);
-        if (ok && n1 > 0) ok = issue_s(1, 1, true, g.T == 2);
-        for (int i = 0; i < g.T && ok; ++i) {
-          ok = issue_pv(i & 1, i, i < 2, true);
-          if (ok && i + 2 < g.T) ok = issue_s(i & 1, i + 2, true, i + 3 == g.T);
-        }
+        u0 += 2 * g.T;
+        if (s_abort) ok = false;
       }
-      u0 += 2 * g.T;
-      ok = __all_sync(0xffffffffu, ok && !s_abort);
+      if (!ok) s_abort = 1;
+      mma_commit(&mma_done[c]);              // every MMA issued above has completed before TMEM is freed
+      mbar_wait_bounded(&mma_done[c], 0);
     }
-    if (!ok) s_abort = 1;
-    if (lane == 0) {
-      mma_commit(&mma_done);                 // every MMA issued above has completed before TMEM is freed
-      mbar_wait_bounded(&mma_done, 0);
+  } else if (warp == 3) {
+    // ---------------------------------------------------------------- page tails (16-bit caches)
+    // The rows of a V tile past the last token inside its page: zeroed (the weights there are zero, and what the
+    // page holds may not be a number), then the tile is passed on.
+    if constexpr (!kE4m3) {
+      uint32_t u = 0, seen = 0;                                // parity of each slot's tail barrier
+      bool ok = true;
+      while (ok && walk.next(a, tiles, it)) {
+        const PcItem g(a, it);
+        const int i = it.r.kl / kKeys - g.kt0;                 // the tile with the first row past the last token
+        const int rows = i >= 0 && i < g.T ? tail_rows(it.r.kl, g.kt0 + i, box) : 0;
+        if (rows > 0) {
+          const uint32_t s = (u + 2 * i + 1) % NS;
+          if (!warp_wait(&tail_full[s], (seen >> s) & 1)) s_abort = 1;
+          seen ^= 1u << s;
+          const int end = it.r.kl & (kKeys - 1);
+          for (int x = lane; x < rows * 8 * DC; x += 32) {
+            const int r = end + x / (8 * DC), q = x % (8 * DC);
+            *reinterpret_cast<uint4*>(smem + L::kKv0 + s * L::kOp + (q >> 3) * kChunkBytes + r * 128 + (q & 7) * 16) =
+                make_uint4(0u, 0u, 0u, 0u);
+          }
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&kv_full[s]);
+        }
+        u += 2 * g.T;
+        if (__any_sync(0xffffffffu, s_abort)) ok = false;
+      }
     }
-  } else if (warp < 4 || warp >= 12) {
+  }
+  } else if (warp >= 12) {
+    regs_down<kOtherRegs>();
     // ---------------------------------------------------------------- helpers: query rows, e4m3 codes to float16
-    const int ht = (warp < 4 ? warp - 2 : warp - 10) * 32 + lane;          // 0 .. 127
+    const int ht = threadIdx.x - 384;                                     // 0 .. 127
     uint32_t u = 0, item = 0;
     bool ok = true;
     while (ok && walk.next(a, tiles, it)) {
@@ -390,7 +426,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
       }
       if constexpr (kE4m3) {
         const uint32_t pitch = ((uint32_t)(box * D) + 127u) & ~127u;
-        const int chunks = D / 16;                              // 16 codes a chunk
+        const int chunks = D / 16, lbox = __ffs(box) - 1;       // 16 codes a chunk
         for (int i = 0; i < 2 * g.T && ok; ++i, ++u) {
           const uint32_t sr = u % NR, s = u % NS;
           if (!warp_wait(&raw_full[sr], (u / NR) & 1)) s_abort = 1;
@@ -399,25 +435,28 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
             ok = false;
             break;
           }
+          if (ht == 0 && g.one_user(i >> 1)) mbar_arrive(&kv_empty[s]);   // for the chain that does not use the tile
           const uint8_t* raw = smem + L::kRaw0 + sr * L::kRaw;
           uint8_t* dst = smem + L::kKv0 + s * L::kOp;
           const int end = it.r.kl - (g.kt0 + (i >> 1)) * kKeys;  // rows from here on are past the last token
-          // thread: chunk ht % (4 DC) of rows ht / (4 DC), + 128 / (4 DC), ...
+          // thread: chunk ht % (4 DC) of rows ht / (4 DC), + 128 / (4 DC), ...; the lanes of the second 64-element
+          // chunk store their halves in the other order, so a quarter-warp's stores cover all banks
           constexpr int CPR = 4 * DC;
           const int c = ht % CPR;
+          const uint32_t flip = (uint32_t)(c >> 2) & 1u;
           if (c < chunks) {
-#pragma unroll 4
+#pragma unroll 8
             for (int r = ht / CPR; r < kKeys; r += kHelpers / CPR) {
-              uint4 x = *reinterpret_cast<const uint4*>(raw + (r / box) * pitch + (r % box) * D + c * 16);
+              uint4 x = *reinterpret_cast<const uint4*>(raw + (r >> lbox) * pitch + (r & (box - 1)) * D + c * 16);
               if (r >= end) x = make_uint4(0u, 0u, 0u, 0u);
               const uint4 lo = make_uint4(e4m3x2_to_f16x2(x.x), e4m3x2_to_f16x2(x.x >> 16), e4m3x2_to_f16x2(x.y),
                                           e4m3x2_to_f16x2(x.y >> 16));
               const uint4 hi = make_uint4(e4m3x2_to_f16x2(x.z), e4m3x2_to_f16x2(x.z >> 16), e4m3x2_to_f16x2(x.w),
                                           e4m3x2_to_f16x2(x.w >> 16));
               uint8_t* d = dst + (c >> 2) * kChunkBytes + r * 128;
-              const int q = (2 * c) & 7;
-              *reinterpret_cast<uint4*>(d + ((q ^ (r & 7)) << 4)) = lo;
-              *reinterpret_cast<uint4*>(d + (((q + 1) ^ (r & 7)) << 4)) = hi;
+              const uint32_t q = ((2 * c) & 7) + flip;
+              *reinterpret_cast<uint4*>(d + ((q ^ (r & 7)) << 4)) = flip ? hi : lo;
+              *reinterpret_cast<uint4*>(d + (((q ^ 1u) ^ (r & 7)) << 4)) = flip ? lo : hi;
             }
           }
           fence_async_smem();
@@ -430,6 +469,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
       }
     }
   } else {
+    regs_up<kSoftmaxRegs>();
     // ---------------------------------------------------------------- softmax (warps 4-7: chain A, 8-11: chain B)
     const int c = (warp - 4) >> 2;
     const int quarter = warp & 3;                          // TMEM lanes this warp may access
@@ -479,60 +519,54 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
         if (any_valid) {
           const int kb = (g.kt0 + (g.wide ? i : 2 * i + c)) * kKeys;
           const bool mask = kb + kKeys - 1 > pos_min;      // some key of the tile may pass a row
-          // The maximum over the upper 64 scores, then over the lower 64, which stay in registers: P of the
-          // lower half goes over columns that have been read, then the upper half is loaded once more.
-          uint32_t r[64];
-          float mx4[4];
-          const float none = sc >= 0.0f ? -INFINITY : INFINITY;
-          mx4[0] = mx4[1] = mx4[2] = mx4[3] = none;
+          uint32_t r[2][64];
+          tmem_ld64_async(s_col, r[0]);
+          tmem_ld64_async(s_col + 64u, r[1]);
+          tmem_ld_wait(r[0]);
+          tmem_ld_wait(r[1]);
+          if (mask) {
 #pragma unroll
-          for (int hf = 1; hf >= 0; --hf) {
-            tmem_ld64_async(s_col + 64u * hf, r);
-            tmem_ld_wait(r);
-            if (mask) {
-#pragma unroll
-              for (int e = 0; e < 64; ++e)
-                if (kb + 64 * hf + e > pos) r[e] = __float_as_uint(hidden);
-            }
-            if (sc >= 0.0f) {
-#pragma unroll
-              for (int e = 0; e < 64; ++e) mx4[e & 3] = fmaxf(mx4[e & 3], __uint_as_float(r[e]));
-            } else {
-#pragma unroll
-              for (int e = 0; e < 64; ++e) mx4[e & 3] = fminf(mx4[e & 3], __uint_as_float(r[e]));
-            }
+            for (int e = 0; e < 128; ++e)
+              if (kb + e > pos) r[e >> 6][e & 63] = __float_as_uint(hidden);
           }
-          const float ext = sc >= 0.0f ? fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]))
-                                       : fminf(fminf(mx4[0], mx4[1]), fminf(mx4[2], mx4[3]));
+          float ext;
+          if (sc >= 0.0f) {
+            float x4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int e = 0; e < 128; e += 8)
+#pragma unroll
+              for (int k = 0; k < 4; ++k) x4[k] = max3(x4[k], __uint_as_float(r[e >> 6][(e & 63) + 2 * k]), __uint_as_float(r[e >> 6][(e & 63) + 2 * k + 1]));
+            ext = fmaxf(fmaxf(x4[0], x4[1]), fmaxf(x4[2], x4[3]));
+          } else {
+            float x4[4] = {INFINITY, INFINITY, INFINITY, INFINITY};
+#pragma unroll
+            for (int e = 0; e < 128; e += 8)
+#pragma unroll
+              for (int k = 0; k < 4; ++k) x4[k] = min3(x4[k], __uint_as_float(r[e >> 6][(e & 63) + 2 * k]), __uint_as_float(r[e >> 6][(e & 63) + 2 * k + 1]));
+            ext = fminf(fminf(x4[0], x4[1]), fminf(x4[2], x4[3]));
+          }
           const float mx = ext * sc - kUp;                 // log2 domain; -inf where the row sees nothing
           const bool grow = mx > m + kGrow;
           const float alpha = grow ? ex2_approx(m - mx) : 1.0f;
           if (grow) m = mx;
           l *= alpha;
           const float neg_m = m == -INFINITY ? 0.0f : -m;
-          float l4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          const uint64_t sc2 = f2_pack(sc, sc), nm2 = f2_pack(neg_m, neg_m);
+          uint64_t l2[2] = {0ull, 0ull};
 #pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
-            if (hf == 1) {
-              tmem_ld64_async(s_col + 64u, r);
-              tmem_ld_wait(r);
-              if (mask) {
-#pragma unroll
-                for (int e = 0; e < 64; ++e)
-                  if (kb + 64 + e > pos) r[e] = __float_as_uint(hidden);
-              }
-            }
+          for (int hf = 0; hf < 2; ++hf) {                 // 64 keys -> 32 packed columns at a time
             uint32_t w[32];
 #pragma unroll
             for (int e = 0; e < 64; e += 2) {
-              const float p0 = ex2_approx(fmaf(__uint_as_float(r[e]), sc, neg_m));
-              const float p1 = ex2_approx(fmaf(__uint_as_float(r[e + 1]), sc, neg_m));
-              l4[(e >> 1) & 3] += p0 + p1;
+              const float2 x = f2_unpack(f2_fma(f2_pack(__uint_as_float(r[hf][e]), __uint_as_float(r[hf][e + 1])), sc2, nm2));
+              const float p0 = ex2_approx(x.x), p1 = ex2_approx(x.y);
+              l2[(e >> 1) & 1] = f2_add(l2[(e >> 1) & 1], f2_pack(p0, p1));
               w[e >> 1] = pack2h<kBf>(p0, p1);
             }
             tmem_st32(s_col + 32u * hf, w);
           }
-          l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
+          const float2 ls = f2_unpack(f2_add(l2[0], l2[1]));
+          l += ls.x + ls.y;
           // O *= alpha where the maximum moved (the whole warp, when any of its rows needs it), once the
           // chain's last PV has completed
           if (i > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
