@@ -71,7 +71,7 @@ __global__ void __launch_bounds__(kPpThreads, 2) paged_prefill_kernel(const __gr
   __shared__ int2 page[2][BK];                       // {block, row in it} of a tile's keys; block -1: nothing there
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
   const int D = a.D;
-  const PgTiles tiles{kPpRows, BK, a.group, 0, 0};
+  const PgTiles tiles{kPpRows, BK, a.group};
 
   // Padding columns [D, DP) of every shared row are zero for the whole kernel (the copies never
   // write them), so they add nothing to Q K^T.

@@ -81,15 +81,14 @@ __device__ __forceinline__ int64_t pg_floor_sum(uint32_t n, uint32_t m, uint32_t
 // Units of tile t of a request with rw = ql * group rows: its last row sees the keys up to position
 // floor(x / group), x = (kl - ql) * group + last row, and so x / (group * bku) + 1 units; at least one,
 // so that rows that see nothing are written too.
-// A request's last tile, when it has at most `few` rows, is cut into units of `few_bku` keys instead.
 struct PgTiles {
-  int rt, bku, group, few, few_bku;
+  int rt, bku, group;
   __device__ __forceinline__ int count(const PgRequest& r) const { return (int)(((int64_t)r.ql * group + rt - 1) / rt); }
   __device__ __forceinline__ int units(const PgRequest& r, int t) const {
     const int rw = r.ql * group;
     const int last = min((t + 1) * rt, rw) - 1;
     const int x = (r.kl - r.ql) * group + last;
-    return x < 0 ? 1 : x / (group * (last - t * rt < few ? few_bku : bku)) + 1;
+    return x < 0 ? 1 : x / (group * bku) + 1;
   }
   // units of tiles [0, t), t <= count
   __device__ __forceinline__ int64_t before(const PgRequest& r, int t) const {

@@ -4,26 +4,29 @@
 //
 // One persistent CTA per SM works through its share of (request, KV head, row tile) items
 // (paged_prefill.cuh).  The query rows of a KV head's group are packed (row = token x group + head), so
-// each key is read once for the whole group.  Two chains S = Q K^T -> softmax -> O += P V run
-// interleaved, each with 128 rows (TMEM lanes), an S buffer and its O in tensor memory and four softmax
-// warps, so one chain's exponentials overlap the other's products:
+// each key is read once for the whole group.  Two chains S = Q K^T -> softmax -> O += P V run side by
+// side, each with 128 rows (TMEM lanes), an S buffer of 128 keys and its O in tensor memory and four
+// softmax warps, so one chain's exponentials overlap the other's products:
 //   wide items (over 128 rows): chain A has rows 0..127 of the tile, chain B rows 128..255, and both
 //     use every K/V tile of 128 keys;
 //   deep items (at most 128 rows: decoding, drafts, the last rows of a prompt): both chains have the
 //     same rows, A takes the even K/V tiles and B the odd ones, and the two results are joined.
+// A chain hands P over in two halves, so the first half of PV runs under the second half's
+// exponentials.  (Two S buffers of 64 keys a chain instead, with the next S computed under the softmax,
+// measured the same: products with N = 64 take as long as with N = 128.)
 // Roles: warp 0 issues the TMA loads (boxes of whole page runs gathered through the block table); one
 // lane each of warps 1 and 2 issues the MMAs of chain A and of chain B (one issuer for both was the
 // limit: its 16 MMAs, four commits and four waits a tile took ~2900 cycles, against 1024 of tensor
 // time); warp 3 zeroes page tails; warps 4-7 and 8-11 are the softmax groups of A and B; warps 12-15
-// gather the query rows and turn e4m3 codes into float16 operands.  The softmax warps take the
-// registers that the others give up (a row's 128 scores stay in registers).
+// gather the query rows and turn e4m3 codes into float16 operands.  The softmax warps take the registers
+// that the others give up, so a row's 128 scores stay in registers.
 // K and V tiles share one ring of shared-memory slots in the order K_0 V_0 K_1 V_1 ...  A page outside
 // the cache, and pages past the last token, are loaded from an out-of-range block coordinate, which
 // TMA fills with zeros; the rows past the last token inside its page are zeroed in shared memory.
 // e4m3: a row of Q is scaled by a power of two that brings its largest element to [1, 2), so float16
 // holds it whatever bfloat16's range had; P is float16 too.
 // Every mbarrier wait is bounded; on a timeout the roles stop, the producer waits for its own copies,
-// the MMA lane for its MMAs, and the CTA frees its TMEM before exiting.
+// the MMA lanes for their MMAs, and the CTA frees its TMEM before exiting.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -40,6 +43,7 @@ namespace {
 
 constexpr int kRows = 128;                 // rows of a chain (TMEM lanes)
 constexpr int kKeys = 128;                 // keys per K/V tile
+constexpr int kHalf = 64;                  // keys whose P is handed over at a time
 constexpr int kTile = 2 * kRows;           // rows of a tile
 constexpr int kThreads = 512;
 constexpr int kHelpers = 128;              // threads of warps 12-15
@@ -73,37 +77,26 @@ __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two) {
   return r;
 }
 
-// What every role derives from an item.
+// What every role derives from an item: key tiles [kt0, kt0 + T), and which of them each chain uses.
 struct PcItem {
   int row0;        // first row of the tile in its request
-  int rw;          // rows of the request
   int rows;        // rows of the tile
   bool wide;
-  int kt0, T;      // key tiles [kt0, kt0 + T)
-  int TA;          // wide: how many of them chain A uses
+  int kt0, T;
+  int TA;          // wide: how many of the tiles chain A uses
   __device__ __forceinline__ PcItem(const PagedArgs& a, const PgItem& it) {
-    rw = it.r.ql * a.group;
     row0 = it.t * kTile;
-    rows = min(kTile, rw - row0);
+    rows = min(kTile, it.r.ql * a.group - row0);
     wide = rows > kRows;
-    const int off = (it.r.kl - it.r.ql) * a.group;
-    const int xb = off + row0 + rows - 1;                       // position of the last row x group
-    const int nb = xb < 0 ? 1 : xb / (a.group * kKeys) + 1;     // key tiles of the tile (one where nothing is seen)
-    if (wide) {
-      kt0 = it.j0;
-      T = it.j1 - it.j0;
-      const int xa = off + row0 + kRows - 1;
-      const int na = xa < 0 ? 0 : xa / (a.group * kKeys) + 1;
-      TA = max(1, min(T, na - kt0));                            // (a tile that it sees nothing of keeps the chains in step)
-    } else {
-      kt0 = 2 * it.j0;
-      T = min(2 * (it.j1 - it.j0), nb - kt0);
-      TA = 0;
-    }
+    kt0 = it.j0;
+    T = it.j1 - it.j0;
+    const int xa = (it.r.kl - it.r.ql) * a.group + row0 + kRows - 1;       // position x group of chain A's last row
+    TA = max(1, min(T, (xa < 0 ? 0 : xa / (a.group * kKeys) + 1) - kt0));  // (a tile that it sees nothing of keeps the chains in step)
   }
-  // tiles of chain c, the first one and the step to the next
+  // tiles of chain c, and its k-th
   __device__ __forceinline__ int count(int c) const { return wide ? (c ? T : TA) : (T - c + 1) >> 1; }
-  // whether one chain alone uses the item's tile i
+  __device__ __forceinline__ int tile(int c, int k) const { return wide ? k : 2 * k + c; }
+  // whether one chain alone uses tile i
   __device__ __forceinline__ bool one_user(int i) const { return !wide || i >= TA; }
 };
 // Rows of key tile kt past the last token that a box of the tile holds together with tokens.
@@ -112,18 +105,14 @@ __device__ __forceinline__ int tail_rows(int kl, int kt, int box) {
   return end > 0 && end < kKeys && in ? box - in : 0;
 }
 
-template <int N> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
-template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-__device__ __forceinline__ float min3(float a, float b, float c) {
-  float r;
-  asm("min.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
+
+template <int N> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 
 template <typename T, bool kE4m3, int DC>
 __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __grid_constant__ CUtensorMap tk,
@@ -140,7 +129,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
   const uint32_t sbase = smem_u32(smem);
   __shared__ uint64_t kv_full[kMaxSlots], kv_empty[kMaxSlots], tail_full[kE4m3 ? 1 : kMaxSlots],
       raw_full[kE4m3 ? kMaxRaw : 1], raw_empty[kE4m3 ? kMaxRaw : 1],
-      q_full, q_empty, s_full[2], p_full[2], pv_done[2], mma_done[2], joined;
+      q_full, q_empty, s_full[2], p_half[2], p_full[2], pv_done[2], mma_done[2], joined;
   __shared__ uint32_t tmem_base_s;
   __shared__ volatile int s_abort;
   __shared__ PgShare share;
@@ -148,8 +137,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
   __shared__ float join_s[2][kRows];             // [chain][row]: maxima, then sums, at the end of a deep item
   __shared__ int8_t qexp_s[2][kE4m3 ? kTile : 1];   // e of a row's Q scale 2^-e, by item parity
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const PgTiles tiles{kTile, kKeys, a.group, kRows, 2 * kKeys};
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const PgTiles tiles{kTile, kKeys, a.group};
   if (threadIdx.x == 0) {
     for (int s = 0; s < NS; ++s) {
       mbar_init(&kv_full[s], kE4m3 ? 4 : 1);
@@ -164,6 +153,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
     mbar_init(&q_empty, 2);
     for (int c = 0; c < 2; ++c) {
       mbar_init(&s_full[c], 1);
+      mbar_init(&p_half[c], 4);
       mbar_init(&p_full[c], 4);
       mbar_init(&pv_done[c], 1);
       mbar_init(&mma_done[c], 1);
@@ -263,26 +253,28 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
     // every copy this CTA issued has landed before it exits (tails: warp 3 has seen theirs)
     for (uint32_t v = u > NF ? u - NF : 0; v < u; ++v) mbar_wait_bounded(&full[v % NF], (v / NF) & 1);
   } else if (warp <= 2) {
-    // ---------------------------------------------------------------- MMA issuers: lane 0 of warp 1 + c, chain c
-    if (lane == 0) {
+    // ---------------------------------------------------------------- MMA issuers: warp 1 + c, chain c
+    {
       const int c = warp - 1;
       const uint32_t tb = tmem + (uint32_t)c * 256u;
       constexpr uint32_t kIdS = idesc_f16(kRows, kKeys, kBf, false);
       const uint32_t id_pv = idesc_f16(kRows, D, kBf, true);
       uint32_t u0 = 0, item = 0;                               // ring position of the item's first tile
-      uint32_t n = 0;                                          // tiles of the chain whose S has been issued
+      uint32_t n = 0;                                          // tiles of the chain so far, all items
       bool ok = true;
       while (ok && walk.next(a, tiles, it)) {
         const PcItem g(a, it);
-        const int count = g.count(c), first = g.wide ? 0 : c, step = g.wide ? 1 : 2;
+        const int count = g.count(c);
         const uint64_t qd = desc_kmajor(sbase + L::kQ0 + (g.wide ? c : 0) * L::kOp);
-        // S of the chain's tile k: item tile first + k * step
-        auto issue_s = [&](int k) -> bool {
-          const uint32_t v = u0 + 2 * (first + k * step), s = v % NS;
-          if (!mbar_wait_bounded(&kv_full[s], (v / NS) & 1)) return false;
-          if (n > 0 && !mbar_wait_bounded(&pv_done[c], (n - 1) & 1)) return false;   // the P it overwrites is used up
+        auto wait_k = [&](int k) -> bool {
+          const uint32_t v = u0 + 2 * g.tile(c, k);
+          return warp_wait(&kv_full[v % NS], (v / NS) & 1);
+        };
+        auto issue_s = [&](int k) {                            // K has landed, the P that S overwrites is used up
+          const uint32_t s = (u0 + 2 * g.tile(c, k)) % NS;
           tc_fence_after();
           const uint64_t kd = desc_kmajor(sbase + L::kKv0 + s * L::kOp);
+          if (elect_one()) {
           // 16 elements = 32 bytes on in both operands, 64 elements one chunk on
           if (D == 64 * DC) {
 #pragma unroll
@@ -297,32 +289,53 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
           mma_commit(&s_full[c]);
           mma_commit(&kv_empty[s]);
           if (k + 1 == count) mma_commit(&q_empty);
-          ++n;
-          return true;
+          }
+          __syncwarp();
         };
-        ok = mbar_wait_bounded(&q_full, item & 1);
+        ok = warp_wait(&q_full, item & 1);
         ++item;
-        if (count == 0 && ok) mbar_arrive(&q_empty);
-        if (count > 0) ok = ok && issue_s(0);
-        for (int k = 0; k < count && ok; ++k) {
-          const uint32_t v = u0 + 2 * (first + k * step) + 1, s = v % NS;
-          ok = mbar_wait_bounded(&kv_full[s], (v / NS) & 1) && mbar_wait_bounded(&p_full[c], (n - 1) & 1);
+        if (count == 0 && ok && lane == 0) mbar_arrive(&q_empty);
+        if (count > 0) {
+          ok = ok && wait_k(0) && (n == 0 || warp_wait(&pv_done[c], (n - 1) & 1));
+          if (ok) issue_s(0);
+        }
+        for (int k = 0; k < count && ok; ++k, ++n) {
+          const uint32_t v = u0 + 2 * g.tile(c, k) + 1, s = v % NS;
+          ok = warp_wait(&kv_full[s], (v / NS) & 1);
+          // (in a deep item the next K may want the slot of this very V: it is waited for after PV)
+          if (ok && g.wide && k + 1 < count) ok = wait_k(k + 1);
+          ok = ok && warp_wait(&p_half[c], n & 1);
           if (!ok) break;
           tc_fence_after();
+          // 16 keys: 8 packed columns of P over the scores, 16 rows of V
           const uint64_t vd = desc_mnmajor(sbase + L::kKv0 + s * L::kOp, kChunkBytes);
+          if (elect_one()) {
 #pragma unroll
-          for (int ks = 0; ks < kKeys / 16; ++ks)   // P: 16 keys = 8 packed columns over the scores
-            mma_f16_ts(tb + 128u, tb + (uint32_t)ks * 8u, vd + ks * 128, id_pv, (k | ks) != 0);
-          mma_commit(&pv_done[c]);
-          mma_commit(&kv_empty[s]);
-          if (k + 1 < count) ok = issue_s(k + 1);
+            for (int ks = 0; ks < kHalf / 16; ++ks) mma_f16_ts(tb + 128u, tb + (uint32_t)ks * 8u, vd + ks * 128, id_pv, (k | ks) != 0);
+          }
+          __syncwarp();
+          ok = warp_wait(&p_full[c], n & 1);
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_one()) {
+#pragma unroll
+            for (int ks = kHalf / 16; ks < kKeys / 16; ++ks) mma_f16_ts(tb + 128u, tb + (uint32_t)ks * 8u, vd + ks * 128, id_pv, 1);
+            mma_commit(&pv_done[c]);
+            mma_commit(&kv_empty[s]);
+          }
+          __syncwarp();
+          if (k + 1 < count) {
+            if (!g.wide) ok = wait_k(k + 1);
+            ok = ok && warp_wait(&pv_done[c], n & 1);
+            if (ok) issue_s(k + 1);
+          }
         }
         u0 += 2 * g.T;
-        if (s_abort) ok = false;
+        if (__any_sync(0xffffffffu, s_abort)) ok = false;
       }
       if (!ok) s_abort = 1;
-      mma_commit(&mma_done[c]);              // every MMA issued above has completed before TMEM is freed
-      mbar_wait_bounded(&mma_done[c], 0);
+      if (elect_one()) mma_commit(&mma_done[c]);              // every MMA issued above has completed before TMEM is freed
+      warp_wait(&mma_done[c], 0);
     }
   } else if (warp == 3) {
     // ---------------------------------------------------------------- page tails (16-bit caches)
@@ -509,80 +522,83 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
       }
       if (sc == 0.0f) sc = 1e-30f;                         // equal weights; a masked score stays -inf below
       const float hidden = sc >= 0.0f ? -INFINITY : INFINITY;
-      float m = -INFINITY, l = 0.0f;
+      const uint64_t sc2 = f2_pack(sc, sc);
+      float m = -INFINITY, l = 0.0f;                       // l: the sum of the P so far, at the scale 2^-m
       for (int i = 0; i < nt; ++i, ++n) {
-        if (__shfl_sync(0xffffffffu, s_abort, 0) || !warp_wait(&s_full[c], n & 1)) {   // warp-uniform
+        if (!warp_wait(&s_full[c], n & 1)) {               // warp-uniform
           ok = false;
           break;
         }
         tc_fence_after();
         if (any_valid) {
-          const int kb = (g.kt0 + (g.wide ? i : 2 * i + c)) * kKeys;
-          const bool mask = kb + kKeys - 1 > pos_min;      // some key of the tile may pass a row
-          uint32_t r[2][64];
+          const int kb = (g.kt0 + g.tile(c, i)) * kKeys;
+          uint32_t r[2][kHalf];
           tmem_ld64_async(s_col, r[0]);
-          tmem_ld64_async(s_col + 64u, r[1]);
+          tmem_ld64_async(s_col + kHalf, r[1]);
           tmem_ld_wait(r[0]);
           tmem_ld_wait(r[1]);
-          if (mask) {
+          if (kb + kKeys - 1 > pos_min) {                  // some key of the tile may pass a row
 #pragma unroll
-            for (int e = 0; e < 128; ++e)
+            for (int e = 0; e < kKeys; ++e)
               if (kb + e > pos) r[e >> 6][e & 63] = __float_as_uint(hidden);
           }
-          float ext;
+          float x4[4] = {hidden, hidden, hidden, hidden};
           if (sc >= 0.0f) {
-            float x4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int e = 0; e < 128; e += 8)
-#pragma unroll
-              for (int k = 0; k < 4; ++k) x4[k] = max3(x4[k], __uint_as_float(r[e >> 6][(e & 63) + 2 * k]), __uint_as_float(r[e >> 6][(e & 63) + 2 * k + 1]));
-            ext = fmaxf(fmaxf(x4[0], x4[1]), fmaxf(x4[2], x4[3]));
+            for (int e = 0; e < kKeys; e += 2)
+              x4[(e >> 1) & 3] = max3(x4[(e >> 1) & 3], __uint_as_float(r[e >> 6][e & 63]), __uint_as_float(r[e >> 6][(e & 63) + 1]));
           } else {
-            float x4[4] = {INFINITY, INFINITY, INFINITY, INFINITY};
 #pragma unroll
-            for (int e = 0; e < 128; e += 8)
-#pragma unroll
-              for (int k = 0; k < 4; ++k) x4[k] = min3(x4[k], __uint_as_float(r[e >> 6][(e & 63) + 2 * k]), __uint_as_float(r[e >> 6][(e & 63) + 2 * k + 1]));
-            ext = fminf(fminf(x4[0], x4[1]), fminf(x4[2], x4[3]));
+            for (int e = 0; e < kKeys; ++e) x4[e & 3] = fminf(x4[e & 3], __uint_as_float(r[e >> 6][e & 63]));
           }
+          const float ext = sc >= 0.0f ? max3(fmaxf(x4[0], x4[1]), x4[2], x4[3]) : fminf(fminf(x4[0], x4[1]), fminf(x4[2], x4[3]));
           const float mx = ext * sc - kUp;                 // log2 domain; -inf where the row sees nothing
+          // The maximum only moves when it grows by more than 2^8: sum and O carry the same factor, so the
+          // result is unchanged, and most tiles need no rescaling.
           const bool grow = mx > m + kGrow;
-          const float alpha = grow ? ex2_approx(m - mx) : 1.0f;
-          if (grow) m = mx;
-          l *= alpha;
+          if (__any_sync(0xffffffffu, grow)) {
+            const float alpha = grow ? ex2_approx(m - mx) : 1.0f;
+            if (grow) m = mx;
+            l *= alpha;
+            if (i > 0) {                                   // O *= alpha, once the chain's last PV has completed
+              if (!warp_wait(&pv_done[c], (n - 1) & 1)) {
+                ok = false;
+                break;
+              }
+              tc_fence_after();
+              for (int x = 0; x < (D + 31) / 32; ++x) {
+                uint32_t o[32];
+                tmem_ld32(o_col + x * 32, o);
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                tmem_st32(o_col + x * 32, o);
+              }
+            }
+          }
           const float neg_m = m == -INFINITY ? 0.0f : -m;
-          const uint64_t sc2 = f2_pack(sc, sc), nm2 = f2_pack(neg_m, neg_m);
+          const uint64_t nm2 = f2_pack(neg_m, neg_m);
           uint64_t l2[2] = {0ull, 0ull};
 #pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {                 // 64 keys -> 32 packed columns at a time
-            uint32_t w[32];
+          for (int hf = 0; hf < 2; ++hf) {
+            uint32_t w[kHalf / 2];
 #pragma unroll
-            for (int e = 0; e < 64; e += 2) {
+            for (int e = 0; e < kHalf; e += 2) {
               const float2 x = f2_unpack(f2_fma(f2_pack(__uint_as_float(r[hf][e]), __uint_as_float(r[hf][e + 1])), sc2, nm2));
               const float p0 = ex2_approx(x.x), p1 = ex2_approx(x.y);
               l2[(e >> 1) & 1] = f2_add(l2[(e >> 1) & 1], f2_pack(p0, p1));
               w[e >> 1] = pack2h<kBf>(p0, p1);
             }
             tmem_st32(s_col + 32u * hf, w);
+            if (hf == 0) {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&p_half[c]);
+            }
           }
           const float2 ls = f2_unpack(f2_add(l2[0], l2[1]));
           l += ls.x + ls.y;
-          // O *= alpha where the maximum moved (the whole warp, when any of its rows needs it), once the
-          // chain's last PV has completed
-          if (i > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
-            if (!warp_wait(&pv_done[c], (n - 1) & 1)) {
-              ok = false;
-              break;
-            }
-            tc_fence_after();
-            for (int x = 0; x < (D + 31) / 32; ++x) {
-              uint32_t o[32];
-              tmem_ld32(o_col + x * 32, o);
-#pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-              tmem_st32(o_col + x * 32, o);
-            }
-          }
+        } else if (lane == 0) {
+          mbar_arrive(&p_half[c]);
         }
         tc_fence_before();
         __syncwarp();
@@ -627,33 +643,37 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
             ml[kTile + trow] = l;
           }
         }
-        // sixteen columns at a time; in a deep item chain A stores the even sixteens and B the odd ones
-        for (int x = g.wide ? 0 : c; x < D / 16; x += g.wide ? 1 : 2) {
-          uint32_t o[16], o2[16];
-          float f[16];
+        // 32 columns at a time; in a deep item chain A stores the even ones and B the odd ones
+        for (int x = g.wide ? 0 : c; x * 32 < D; x += g.wide ? 1 : 2) {
+          uint32_t o[32], o2[32];
 #pragma unroll
-          for (int e = 0; e < 16; ++e) o[e] = o2[e] = 0u;
-          if (nt > 0) tmem_ld16_async(o_col + x * 16, o);
-          if (has_other) tmem_ld16_async((o_col ^ 256u) + x * 16, o2);
+          for (int e = 0; e < 32; ++e) o[e] = o2[e] = 0u;
+          if (nt > 0) tmem_ld32_async(o_col + x * 32, o);
+          if (has_other) tmem_ld32_async((o_col ^ 256u) + x * 32, o2);
           tmem_ld_wait(o);
           tmem_ld_wait(o2);
+          float f[32];
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
+          for (int e = 0; e < 32; ++e) {
             float y = __uint_as_float(o[e]);
             if (!g.wide) y = y * w_own + __uint_as_float(o2[e]) * w_other;
             f[e] = y * fin;
           }
           if (!valid) continue;
-          if (whole) {
-            uint32_t w[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) w[e] = pack2h<std::is_same<T, __nv_bfloat16>::value>(f[2 * e], f[2 * e + 1]);
-            *reinterpret_cast<uint4*>(og + x * 16) = make_uint4(w[0], w[1], w[2], w[3]);
-            *reinterpret_cast<uint4*>(og + x * 16 + 8) = make_uint4(w[4], w[5], w[6], w[7]);
-          } else {
+          for (int q = 0; q < 4; ++q) {
+            if (x * 32 + q * 8 >= D) break;
+            if (whole) {
+              uint32_t w[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              *reinterpret_cast<float4*>(po + x * 16 + 4 * e) = make_float4(f[4 * e], f[4 * e + 1], f[4 * e + 2], f[4 * e + 3]);
+              for (int e = 0; e < 4; ++e)
+                w[e] = pack2h<std::is_same<T, __nv_bfloat16>::value>(f[8 * q + 2 * e], f[8 * q + 2 * e + 1]);
+              *reinterpret_cast<uint4*>(og + x * 32 + q * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+            } else {
+              float4* d4 = reinterpret_cast<float4*>(po + x * 32 + q * 8);
+              d4[0] = make_float4(f[8 * q], f[8 * q + 1], f[8 * q + 2], f[8 * q + 3]);
+              d4[1] = make_float4(f[8 * q + 4], f[8 * q + 5], f[8 * q + 6], f[8 * q + 7]);
+            }
           }
         }
       }
