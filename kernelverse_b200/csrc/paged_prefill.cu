@@ -296,7 +296,7 @@ __global__ void __launch_bounds__(kPpThreads, 2) paged_prefill_kernel(const __gr
     l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
     const float vsc = kE4m3 ? __ldg(a.v_scale + it.h) : 1.0f;   // V codes were used unscaled
     if (it.whole()) {
-      const float inv0 = l0 > 0.0f ? vsc / l0 : 0.0f, inv1 = l1 > 0.0f ? vsc / l1 : 0.0f;
+      const float inv0 = l0 == 0.0f ? 0.0f : vsc / l0, inv1 = l1 == 0.0f ? 0.0f : vsc / l1;
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
         const int gr = hf ? gr1 : gr0;
@@ -377,7 +377,7 @@ __global__ void __launch_bounds__(256) paged_prefill_merge_kernel(const __grid_c
     }
     const int gr = cut.x + row, tok = gr / a.group, hd = cut.z * a.group + (gr - tok * a.group);
     const int64_t orow = (int64_t)(r.q0 + tok) * a.hq + hd;
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     if (a.lse && lane == 0) a.lse[orow] = (m + log2f(l)) * kPgLn2;
     if (col < a.D) {
       T* p = reinterpret_cast<T*>(a.out) + orow * a.D + col;

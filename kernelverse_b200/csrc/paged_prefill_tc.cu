@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
   if (warp == 0) {
     // ---------------------------------------------------------------- TMA producer
     // A tile is kKeys / box boxes of `box` keys, each inside one page; lane l serves box l % boxes.
-    const int boxes = kKeys / box, lboxes = __ffs(boxes) - 1;
+    const int boxes = kKeys / box;
     const int bx = lane & (boxes - 1);
     constexpr int NF = kE4m3 ? NR : NS;                        // ring the copies go to
     uint64_t* const full = kE4m3 ? raw_full : kv_full;
@@ -236,14 +236,20 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
           }
           if (lane == 0) mbar_arrive_expect_tx(bar, bytes);
           __syncwarp();
-          if constexpr (kE4m3) {
-            const uint32_t pitch = ((uint32_t)(box * D) + 127u) & ~127u;
-            if (lane < boxes) tma_load_4d(sbase + L::kRaw0 + s * L::kRaw + bx * pitch, map, 0, it.h, in, phys, bar);
-          } else {
-            for (int x = lane; x < DC * boxes; x += 32) {
-              const int c = x >> lboxes;
-              tma_load_4d(sbase + L::kKv0 + s * L::kOp + c * kChunkBytes + bx * box * 128, map, c * 64, it.h, in, phys, bar);
+          // box by box in converged code (issued by the lanes of the boxes instead, each took ~105 cycles)
+          for (int x = 0; x < boxes; ++x) {
+            const int p = __shfl_sync(0xffffffffu, phys, x), r = __shfl_sync(0xffffffffu, in, x);
+            if (elect_one()) {
+              if constexpr (kE4m3) {
+                const uint32_t pitch = ((uint32_t)(box * D) + 127u) & ~127u;
+                tma_load_4d(sbase + L::kRaw0 + s * L::kRaw + x * pitch, map, 0, it.h, r, p, bar);
+              } else {
+#pragma unroll
+                for (int c = 0; c < DC; ++c)
+                  tma_load_4d(sbase + L::kKv0 + s * L::kOp + c * kChunkBytes + x * box * 128, map, c * 64, it.h, r, p, bar);
+              }
             }
+            __syncwarp();
           }
         }
         phys = phys_next;
@@ -629,7 +635,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
       if (ok && any_valid) {
         const float vsc = kE4m3 ? __ldg(a.v_scale + it.h) : 1.0f;
         const bool whole = it.whole();
-        const float fin = whole ? (l > 0.0f ? vsc / l : 0.0f) : vsc;
+        const float fin = whole ? (l == 0.0f ? 0.0f : vsc / l) : vsc;
         const int64_t slot = 2 * (int64_t)blockIdx.x + (it.j0 == 0 ? 1 : 0);
         const int64_t orow = (int64_t)(it.r.q0 + tok) * a.hq + it.h * a.group + (gr - tok * a.group);
         T* og = reinterpret_cast<T*>(a.out) + orow * D;
