@@ -10,7 +10,6 @@ tensors through the GPU kernel.
 """
 from __future__ import annotations
 
-from contextlib import nullcontext
 from functools import lru_cache
 from typing import Optional, Tuple
 
@@ -56,12 +55,25 @@ def _paged_prefill_workspace(head_dim: int) -> int:
     return _lib.lib().kvb_paged_prefill_attention_workspace_size(head_dim)
 
 
-def _on(dev: torch.device):
-    """Makes ``dev`` the current device for a launch; nothing to do where it already is."""
-    return _HERE if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+# The rotary, paged-append and paged-prefill operators are called once or twice a layer in a decode step,
+# where the host's time per call is what counts: they check their arguments in one expression, name what
+# is wrong only when something is, and ask torch for little else than their outputs.
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+_INDEX = {torch.int32: _lib.I32, torch.int64: _lib.I64}
+_CACHE = {**_DT, torch.uint8: _lib.E4M3}
 
 
-_HERE = nullcontext()
+def _device_of(what: str, *ts) -> int:
+    """The index of the CUDA device that every tensor is on."""
+    dev = ts[0].get_device()
+    for t in ts:
+        if t is not None and t.get_device() != dev:
+            dev = -1
+    if dev < 0:
+        _cuda(*ts)            # names what is wrong
+        raise ValueError(f"{what}: tensors on different devices")
+    return dev
 
 
 _workspaces = {}
@@ -341,31 +353,23 @@ def rope_cos_sin(max_positions: int, rotary_dim: int, base: float = 10000.0, dev
     return table if device is None else table.to(device)
 
 
-def _heads(what: str, name: str, t: torch.Tensor) -> torch.Tensor:
-    """A [tokens, heads, head_dim] tensor whose last dimension is contiguous (views of a fused
-    projection stay views)."""
-    if t.dim() != 3:
-        raise ValueError(f"{what}: {name} must be [tokens, heads, head_dim]")
-    return t if t.stride(2) == 1 else t.contiguous()
-
-
-def _rope_args(what, q, k, positions, cos_sin, q_weight, k_weight):
-    """Checks shared by the two rope entry points; returns (q, k, positions, cos_sin, weights)."""
-    q, k = _heads(what, "q", q), _heads(what, "k", k)
-    t, hq, d = q.shape
+def _rope_refusal(what, q, k, positions, cos_sin, q_weight, k_weight):
+    if q.dim() != 3 or k.dim() != 3:
+        raise ValueError(f"{what}: q and k must be [tokens, heads, head_dim]")
+    t, _, d = q.shape
     if k.shape[0] != t or k.shape[2] != d:
         raise ValueError(f"{what}: q and k must have the same tokens and head_dim")
-    if k.dtype != q.dtype:
-        raise TypeError(f"{what}: q and k must share a dtype")
-    if positions.dim() != 1 or positions.shape[0] != t:
+    if q.dtype not in (torch.float32, torch.float16, torch.bfloat16) or k.dtype != q.dtype:
+        raise TypeError(f"{what}: q and k must share a dtype of float32, float16 and bfloat16")
+    if positions.shape != (t,):
         raise ValueError(f"{what}: positions must be [tokens]")
+    if positions.dtype not in _INDEX:
+        raise TypeError(f"{what}: positions must be int32 or int64")
     if cos_sin.dim() != 2 or cos_sin.dtype != torch.float32:
         raise TypeError(f"{what}: cos_sin must be float32 [max_positions, rotary_dim]")
     for w in (q_weight, k_weight):
         if w is not None and (w.shape != (d,) or w.dtype != q.dtype):
             raise ValueError(f"{what}: norm weights must be [head_dim] of q's dtype")
-    return (q, k, positions.contiguous(), cos_sin.contiguous(), None if q_weight is None else q_weight.contiguous(),
-            None if k_weight is None else k_weight.contiguous())
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor,
@@ -379,30 +383,34 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, cos_
     as halves (n, n + R/2) or, ``interleaved``, as neighbours (2n, 2n + 1).  float32 arithmetic with one
     rounding.  Returns new contiguous ``(q_out, k_out)``, as :func:`batched_prefill_attention` takes
     them.  A position outside the table gives NaN heads and sets device status bit 1."""
-    dev = _cuda(q, k, positions, cos_sin, q_weight, k_weight)
-    q, k, positions, cos_sin, q_weight, k_weight = _rope_args("qk_norm_rope", q, k, positions, cos_sin, q_weight, k_weight)
+    dev = _device_of("qk_norm_rope", q, k, positions, cos_sin, q_weight, k_weight)
+    if dev != _current_device():
+        with torch.cuda.device(dev):
+            return qk_norm_rope(q, k, positions, cos_sin, q_weight, k_weight, eps, interleaved)
+    _rope_refusal("qk_norm_rope", q, k, positions, cos_sin, q_weight, k_weight)
     t, hq, d = q.shape
-    hkv = k.shape[1]
-    with _on(dev):
-        q_out = torch.empty((t, hq, d), dtype=q.dtype, device=dev)
-        k_out = torch.empty((t, hkv, d), dtype=q.dtype, device=dev)
-        call("kvb_qk_norm_rope", q.data_ptr(), k.data_ptr(), kvb_dtype(q.dtype), q.stride(0), q.stride(1), k.stride(0),
-             k.stride(1), positions.data_ptr(), _index_dtype(positions), cos_sin.data_ptr(), cos_sin.shape[0],
-             cos_sin.shape[1], 1 if interleaved else 0, _ptr(q_weight), _ptr(k_weight), float(eps), t, hq, hkv, d,
-             q_out.data_ptr(), k_out.data_ptr(), _stream(dev))
+    (qt, qh, q1), (kt, kh, k1) = q.stride(), k.stride()
+    if q1 != 1 or k1 != 1:
+        q, k = q.contiguous(), k.contiguous()
+        (qt, qh, _), (kt, kh, _) = q.stride(), k.stride()
+    positions, cos_sin = positions.contiguous(), cos_sin.contiguous()
+    q_weight, k_weight = (None if w is None else w.contiguous() for w in (q_weight, k_weight))
+    q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
+    call("kvb_qk_norm_rope", q.data_ptr(), k.data_ptr(), _DT[q.dtype], qt, qh, kt, kh, positions.data_ptr(),
+         _INDEX[positions.dtype], cos_sin.data_ptr(), *cos_sin.shape, 1 if interleaved else 0, _ptr(q_weight), _ptr(k_weight),
+         eps, t, hq, k.shape[1], d, q_out.data_ptr(), k_out.data_ptr(), _raw_stream(dev))
     return q_out, k_out
 
 
 def _paged_blocks(what: str, name: str, cache: torch.Tensor) -> int:
     """Checks a paged cache that is used in place ([num_blocks, block_size, Hkv, D], each block
     contiguous) and returns its block stride in elements."""
-    if cache.dim() != 4:
-        raise ValueError(f"{what}: {name} must be [num_blocks, block_size, num_kv_heads, head_dim]")
     nb, bs, h, d = cache.shape
-    want = (h * d, d, 1)
-    if any(n > 1 and s != w for n, s, w in zip((bs, h, d), cache.stride()[1:], want)):
+    s0, s1, s2, s3 = cache.stride()
+    if (s3 != 1 and d > 1) or (s2 != d and h > 1) or (s1 != h * d and bs > 1):
         raise ValueError(f"{what}: the blocks of {name} must be contiguous")
-    return cache.stride(0) if nb > 1 else bs * h * d
+    return s0 if nb > 1 else bs * h * d
 
 
 def _cache_scales(what, cache_dtype, hkv, k_scale, v_scale):
@@ -415,7 +423,9 @@ def _cache_scales(what, cache_dtype, hkv, k_scale, v_scale):
         raise ValueError(f"{what}: an e4m3 cache needs k_scale and v_scale")
     if k_scale.numel() != hkv or v_scale.numel() != hkv:
         raise ValueError(f"{what}: k_scale and v_scale must have one entry per KV head")
-    return k_scale.to(torch.float32).contiguous(), v_scale.to(torch.float32).contiguous()
+    if k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
+        k_scale, v_scale = k_scale.to(torch.float32), v_scale.to(torch.float32)
+    return k_scale.contiguous(), v_scale.contiguous()
 
 
 def rope_paged_kv_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -433,31 +443,39 @@ def rope_paged_kv_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_ca
     A negative slot keeps its token out of the cache; slots must be distinct.  Slots or positions out of
     range set device status bit 1."""
     what = "rope_paged_kv_append"
-    dev = _cuda(q, k, v, k_cache, v_cache, slot_mapping, positions, cos_sin, k_scale, v_scale, q_weight, k_weight)
-    q, k, positions, cos_sin, q_weight, k_weight = _rope_args(what, q, k, positions, cos_sin, q_weight, k_weight)
-    v = _heads(what, "v", v)
+    dev = _device_of(what, q, k, v, k_cache, v_cache, slot_mapping, positions, cos_sin, k_scale, v_scale, q_weight, k_weight)
+    if dev != _current_device():
+        with torch.cuda.device(dev):
+            return rope_paged_kv_append(q, k, v, k_cache, v_cache, slot_mapping, positions, cos_sin, k_scale, v_scale,
+                                        q_weight, k_weight, eps, interleaved)
+    _rope_refusal(what, q, k, positions, cos_sin, q_weight, k_weight)
     t, hq, d = q.shape
     hkv = k.shape[1]
     if v.shape != k.shape or v.dtype != k.dtype:
         raise ValueError(f"{what}: v must have k's shape and dtype")
-    if v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype or k_cache.shape[2:] != (hkv, d):
+    if v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype or k_cache.dim() != 4 or k_cache.shape[2:] != (hkv, d):
         raise ValueError(f"{what}: caches must both be [num_blocks, block_size, num_kv_heads, head_dim]")
-    cdt = _cache_kvb_dtype(k_cache)
+    cdt = _CACHE.get(k_cache.dtype)
     if cdt != _lib.E4M3 and k_cache.dtype != q.dtype:
         raise TypeError(f"{what}: caches hold q's dtype or e4m3 codes")
     ks, vs = _paged_blocks(what, "k_cache", k_cache), _paged_blocks(what, "v_cache", v_cache)
-    if slot_mapping.dim() != 1 or slot_mapping.shape[0] != t:
+    if slot_mapping.shape != (t,):
         raise ValueError(f"{what}: slot_mapping must be [tokens]")
-    with _on(dev):
-        k_scale, v_scale = _cache_scales(what, cdt, hkv, k_scale, v_scale)
-        slot_mapping = slot_mapping.contiguous()
-        q_out = torch.empty((t, hq, d), dtype=q.dtype, device=dev)
-        call("kvb_rope_paged_kv_append", q.data_ptr(), k.data_ptr(), v.data_ptr(), kvb_dtype(q.dtype), q.stride(0),
-             q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1), positions.data_ptr(), _index_dtype(positions),
-             slot_mapping.data_ptr(), _index_dtype(slot_mapping), cos_sin.data_ptr(), cos_sin.shape[0], cos_sin.shape[1],
-             1 if interleaved else 0, _ptr(q_weight), _ptr(k_weight), float(eps), t, hq, hkv, d, k_cache.data_ptr(),
-             v_cache.data_ptr(), cdt, k_cache.shape[1], k_cache.shape[0], ks, vs, _ptr(k_scale), _ptr(v_scale),
-             q_out.data_ptr(), _stream(dev))
+    if slot_mapping.dtype not in _INDEX:
+        raise TypeError(f"{what}: slot_mapping must be int32 or int64")
+    k_scale, v_scale = _cache_scales(what, cdt, hkv, k_scale, v_scale)
+    (qt, qh, q1), (kt, kh, k1), (vt, vh, v1) = q.stride(), k.stride(), v.stride()
+    if q1 != 1 or k1 != 1 or v1 != 1:
+        q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
+        (qt, qh, _), (kt, kh, _), (vt, vh, _) = q.stride(), k.stride(), v.stride()
+    positions, cos_sin, slot_mapping = positions.contiguous(), cos_sin.contiguous(), slot_mapping.contiguous()
+    q_weight, k_weight = (None if w is None else w.contiguous() for w in (q_weight, k_weight))
+    q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    call("kvb_rope_paged_kv_append", q.data_ptr(), k.data_ptr(), v.data_ptr(), _DT[q.dtype], qt, qh, kt, kh, vt, vh,
+         positions.data_ptr(), _INDEX[positions.dtype], slot_mapping.data_ptr(), _INDEX[slot_mapping.dtype],
+         cos_sin.data_ptr(), *cos_sin.shape, 1 if interleaved else 0, _ptr(q_weight), _ptr(k_weight), eps, t, hq, hkv, d,
+         k_cache.data_ptr(), v_cache.data_ptr(), cdt, k_cache.shape[1], k_cache.shape[0], ks, vs, _ptr(k_scale),
+         _ptr(v_scale), q_out.data_ptr(), _raw_stream(dev))
     return q_out
 
 
@@ -605,44 +623,49 @@ def paged_prefill_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     sums of exp [total_q, Hq] float32.  A query that sees no key (q_len > seq_len) gives 0 and -inf; rows
     past the last request are left as they were.  Equal inputs give equal outputs."""
     what = "paged_prefill_attention"
-    dev = _cuda(q, k_cache, v_cache, qo_indptr, seq_lens, block_table, k_scale, v_scale, out)
-    if q.dim() != 3:
-        raise ValueError(f"{what}: q must be [total_q, num_q_heads, head_dim]")
+    dev = _device_of(what, q, k_cache, v_cache, qo_indptr, seq_lens, block_table, k_scale, v_scale, out)
+    if dev != _current_device():
+        with torch.cuda.device(dev):
+            return paged_prefill_attention(q, k_cache, v_cache, qo_indptr, seq_lens, block_table, scale, k_scale, v_scale,
+                                           max_seq_len, return_lse, out, _variant)
+    if q.dim() != 3 or q.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        raise ValueError(f"{what}: q must be [total_q, num_q_heads, head_dim] of float32, float16 or bfloat16")
     tq, hq, d = q.shape
     if v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype or k_cache.dim() != 4 or k_cache.shape[3] != d:
         raise ValueError(f"{what}: caches must both be [num_blocks, block_size, num_kv_heads, head_dim]")
     nb, bs, hkv, _ = k_cache.shape
-    cdt = _cache_kvb_dtype(k_cache)
+    cdt = _CACHE.get(k_cache.dtype)
     if cdt != _lib.E4M3 and k_cache.dtype != q.dtype:
         raise TypeError(f"{what}: caches hold q's dtype or e4m3 codes")
     ks, vs = _paged_blocks(what, "k_cache", k_cache), _paged_blocks(what, "v_cache", v_cache)
-    if qo_indptr.dtype != torch.int32 or block_table.dtype != torch.int32:
-        raise TypeError(f"{what}: qo_indptr and block_table must be int32")
+    if qo_indptr.dtype != torch.int32 or block_table.dtype != torch.int32 or seq_lens.dtype not in _INDEX:
+        raise TypeError(f"{what}: qo_indptr and block_table must be int32, seq_lens int32 or int64")
     b = seq_lens.shape[0] if seq_lens.dim() == 1 else -1
-    if qo_indptr.dim() != 1 or qo_indptr.shape[0] != b + 1 or block_table.dim() != 2 or block_table.shape[0] != b:
+    if qo_indptr.shape != (b + 1,) or block_table.dim() != 2 or block_table.shape[0] != b:
         raise ValueError(f"{what}: qo_indptr [batch + 1], seq_lens [batch], block_table [batch, max_blocks]")
-    if max_seq_len is None:
-        max_seq_len = block_table.shape[1] * bs
-    scale = d ** -0.5 if scale is None else scale
-    if q.stride(2) != 1 or q.stride(1) != d or (q.stride(0) * q.element_size()) % 16 or q.data_ptr() % 16:
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
+        raise ValueError(f"{what}: out must be a contiguous tensor of q's shape and dtype")
+    k_scale, v_scale = _cache_scales(what, cdt, hkv, k_scale, v_scale)
+    qt, qh, q1 = q.stride()
+    if q1 != 1 or qh != d or (qt * q.element_size()) % 16 or q.data_ptr() % 16:
         q = q.contiguous()
-    with _on(dev):
-        k_scale, v_scale = _cache_scales(what, cdt, hkv, k_scale, v_scale)
-        qo_indptr, seq_lens = qo_indptr.contiguous(), seq_lens.contiguous()
-        if block_table.stride(1) != 1 or block_table.stride(0) < block_table.shape[1]:
-            block_table = block_table.contiguous()
-        if out is None:
-            out = torch.empty((tq, hq, d), dtype=q.dtype, device=dev)
-        elif out.shape != (tq, hq, d) or out.dtype != q.dtype or not out.is_contiguous():
-            raise ValueError(f"{what}: out must be a contiguous tensor of q's shape and dtype")
-        lse = torch.empty((tq, hq), dtype=torch.float32, device=dev) if return_lse else None
-        # per call, from the caching allocator: calls on other streams and captured graphs do not share it
-        ws = torch.empty(_paged_prefill_workspace(d), dtype=torch.uint8, device=dev)
-        call("kvb_paged_prefill_attention_variant", q.data_ptr(), kvb_dtype(q.dtype), q.stride(0), k_cache.data_ptr(),
-             v_cache.data_ptr(), cdt, ks, vs, _ptr(k_scale), _ptr(v_scale), qo_indptr.data_ptr(), seq_lens.data_ptr(),
-             _index_dtype(seq_lens), block_table.data_ptr(), block_table.stride(0), b, tq, hq, hkv, d, bs, nb,
-             int(max_seq_len), float(scale), out.data_ptr(), _ptr(lse), int(_variant), ws.data_ptr(), ws.numel(),
-             _stream(dev))
+        qt = q.stride(0)
+    t0, t1 = block_table.stride()
+    if t1 != 1 or t0 < block_table.shape[1]:
+        block_table = block_table.contiguous()
+        t0 = block_table.shape[1]
+    qo_indptr, seq_lens = qo_indptr.contiguous(), seq_lens.contiguous()
+    lse = q.new_empty((tq, hq), dtype=torch.float32) if return_lse else None
+    # per call, from the caching allocator: calls on other streams and captured graphs do not share it
+    ws_bytes = _paged_prefill_workspace(d)
+    ws = q.new_empty((ws_bytes,), dtype=torch.uint8)
+    call("kvb_paged_prefill_attention_variant", q.data_ptr(), _DT[q.dtype], qt, k_cache.data_ptr(), v_cache.data_ptr(), cdt,
+         ks, vs, _ptr(k_scale), _ptr(v_scale), qo_indptr.data_ptr(), seq_lens.data_ptr(), _INDEX[seq_lens.dtype],
+         block_table.data_ptr(), t0, b, tq, hq, hkv, d, bs, nb,
+         block_table.shape[1] * bs if max_seq_len is None else max_seq_len, d ** -0.5 if scale is None else scale,
+         out.data_ptr(), _ptr(lse), _variant, ws.data_ptr(), ws_bytes, _raw_stream(dev))
     return (out, lse) if return_lse else out
 
 
