@@ -67,12 +67,12 @@ _CACHE = {**_DT, torch.uint8: _lib.E4M3}
 def _device_of(what: str, *ts) -> int:
     """The index of the CUDA device that every tensor is on."""
     dev = ts[0].get_device()
-    for t in ts:
-        if t is not None and t.get_device() != dev:
-            dev = -1
     if dev < 0:
         _cuda(*ts)            # names what is wrong
-        raise ValueError(f"{what}: tensors on different devices")
+    for t in ts:
+        if t is not None and t.get_device() != dev:
+            _cuda(*ts)
+            raise ValueError(f"{what}: tensors on different devices")
     return dev
 
 
@@ -353,7 +353,18 @@ def rope_cos_sin(max_positions: int, rotary_dim: int, base: float = 10000.0, dev
     return table if device is None else table.to(device)
 
 
-def _rope_refusal(what, q, k, positions, cos_sin, q_weight, k_weight):
+_FLOATS = frozenset((torch.float32, torch.float16, torch.bfloat16))
+
+
+def _rope_check(what, q, k, positions, cos_sin, q_weight, k_weight):
+    """(tokens, q heads, KV heads, head_dim), or the refusal of what does not fit."""
+    qs, ks, dt = q.shape, k.shape, q.dtype
+    if (len(qs) == 3 and len(ks) == 3 and ks[0] == qs[0] and ks[2] == qs[2] and dt in _FLOATS and k.dtype == dt
+            and positions.shape == qs[:1] and positions.dtype in _INDEX and cos_sin.dim() == 2
+            and cos_sin.dtype == torch.float32
+            and (q_weight is None or (q_weight.shape == qs[2:] and q_weight.dtype == dt))
+            and (k_weight is None or (k_weight.shape == qs[2:] and k_weight.dtype == dt))):
+        return qs[0], qs[1], ks[1], qs[2]
     if q.dim() != 3 or k.dim() != 3:
         raise ValueError(f"{what}: q and k must be [tokens, heads, head_dim]")
     t, _, d = q.shape
@@ -370,6 +381,7 @@ def _rope_refusal(what, q, k, positions, cos_sin, q_weight, k_weight):
     for w in (q_weight, k_weight):
         if w is not None and (w.shape != (d,) or w.dtype != q.dtype):
             raise ValueError(f"{what}: norm weights must be [head_dim] of q's dtype")
+    raise ValueError(f"{what}: bad arguments")
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor,
@@ -387,19 +399,21 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, cos_
     if dev != _current_device():
         with torch.cuda.device(dev):
             return qk_norm_rope(q, k, positions, cos_sin, q_weight, k_weight, eps, interleaved)
-    _rope_refusal("qk_norm_rope", q, k, positions, cos_sin, q_weight, k_weight)
-    t, hq, d = q.shape
+    t, hq, hkv, d = _rope_check("qk_norm_rope", q, k, positions, cos_sin, q_weight, k_weight)
     (qt, qh, q1), (kt, kh, k1) = q.stride(), k.stride()
     if q1 != 1 or k1 != 1:
         q, k = q.contiguous(), k.contiguous()
         (qt, qh, _), (kt, kh, _) = q.stride(), k.stride()
     positions, cos_sin = positions.contiguous(), cos_sin.contiguous()
-    q_weight, k_weight = (None if w is None else w.contiguous() for w in (q_weight, k_weight))
+    if q_weight is not None:
+        q_weight = q_weight.contiguous()
+    if k_weight is not None:
+        k_weight = k_weight.contiguous()
     q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
     k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
     call("kvb_qk_norm_rope", q.data_ptr(), k.data_ptr(), _DT[q.dtype], qt, qh, kt, kh, positions.data_ptr(),
          _INDEX[positions.dtype], cos_sin.data_ptr(), *cos_sin.shape, 1 if interleaved else 0, _ptr(q_weight), _ptr(k_weight),
-         eps, t, hq, k.shape[1], d, q_out.data_ptr(), k_out.data_ptr(), _raw_stream(dev))
+         eps, t, hq, hkv, d, q_out.data_ptr(), k_out.data_ptr(), _raw_stream(dev))
     return q_out, k_out
 
 
@@ -448,9 +462,7 @@ def rope_paged_kv_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_ca
         with torch.cuda.device(dev):
             return rope_paged_kv_append(q, k, v, k_cache, v_cache, slot_mapping, positions, cos_sin, k_scale, v_scale,
                                         q_weight, k_weight, eps, interleaved)
-    _rope_refusal(what, q, k, positions, cos_sin, q_weight, k_weight)
-    t, hq, d = q.shape
-    hkv = k.shape[1]
+    t, hq, hkv, d = _rope_check(what, q, k, positions, cos_sin, q_weight, k_weight)
     if v.shape != k.shape or v.dtype != k.dtype:
         raise ValueError(f"{what}: v must have k's shape and dtype")
     if v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype or k_cache.dim() != 4 or k_cache.shape[2:] != (hkv, d):
@@ -469,7 +481,10 @@ def rope_paged_kv_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_ca
         q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
         (qt, qh, _), (kt, kh, _), (vt, vh, _) = q.stride(), k.stride(), v.stride()
     positions, cos_sin, slot_mapping = positions.contiguous(), cos_sin.contiguous(), slot_mapping.contiguous()
-    q_weight, k_weight = (None if w is None else w.contiguous() for w in (q_weight, k_weight))
+    if q_weight is not None:
+        q_weight = q_weight.contiguous()
+    if k_weight is not None:
+        k_weight = k_weight.contiguous()
     q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
     call("kvb_rope_paged_kv_append", q.data_ptr(), k.data_ptr(), v.data_ptr(), _DT[q.dtype], qt, qh, kt, kh, vt, vh,
          positions.data_ptr(), _INDEX[positions.dtype], slot_mapping.data_ptr(), _INDEX[slot_mapping.dtype],
