@@ -15,6 +15,8 @@
 // whose elements pair up, so the rotation needs no exchange and the norm one shuffle tree; a lane
 // keeps the same element range for every head it serves, so cos, sin and the weights are loaded
 // once per token and lane.
+#include <type_traits>
+
 #include "kvb_common.cuh"
 #include "kvb_async.cuh"
 
@@ -23,6 +25,7 @@ namespace {
 
 constexpr unsigned int kStatusBadRopeIndex = 2u;   // a position or slot out of range
 constexpr int kRopeThreads = 256;
+constexpr int kRopeHeads = 2, kRopeBlocks = 4;   // heads a team, blocks an SM for long inputs
 
 struct RopeArgs {
   const void* q;
@@ -54,16 +57,19 @@ template <typename T, int V> struct VecN {
   static constexpr int kBytes = V * (int)sizeof(T);
   static constexpr int kWords = kBytes / 4;
   uint32_t w[kWords];
+  template <bool kOnce = false>            // kOnce: read-once data, not kept in L1 beside the table's rows
   __device__ __forceinline__ void load(const T* p) {
     if constexpr (kWords % 4 == 0) {
 #pragma unroll
       for (int i = 0; i < kWords / 4; ++i) {
-        const uint4 x = __ldg(reinterpret_cast<const uint4*>(p) + i);
+        const uint4* q = reinterpret_cast<const uint4*>(p) + i;
+        const uint4 x = kOnce ? __ldcs(q) : __ldg(q);
         w[4 * i] = x.x; w[4 * i + 1] = x.y; w[4 * i + 2] = x.z; w[4 * i + 3] = x.w;
       }
     } else {
       static_assert(kWords == 2, "8- or 16-byte vectors");
-      const uint2 x = __ldg(reinterpret_cast<const uint2*>(p));
+      const uint2* q = reinterpret_cast<const uint2*>(p);
+      const uint2 x = kOnce ? __ldcs(q) : __ldg(q);
       w[0] = x.x; w[1] = x.y;
     }
   }
@@ -76,49 +82,82 @@ template <typename T, int V> struct VecN {
       *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
     }
   }
-  __device__ __forceinline__ void unpack(float (&f)[V]) const {
-    const T* e = reinterpret_cast<const T*>(w);
+  // The elements as packed float32 pairs, and back with one rounding.
+  __device__ __forceinline__ void unpack(uint64_t (&f)[V / 2]) const {
 #pragma unroll
-    for (int i = 0; i < V; ++i) f[i] = Elem<T>::to_f(e[i]);
+    for (int i = 0; i < V / 2; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        f[i] = f2_pack(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+      } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        f[i] = f2_pack(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+      } else {
+        const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        f[i] = f2_pack(x.x, x.y);
+      }
+    }
   }
-  __device__ __forceinline__ void pack(const float (&f)[V]) {
-    T* e = reinterpret_cast<T*>(w);
+  __device__ __forceinline__ void pack(const uint64_t (&f)[V / 2]) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) e[i] = Elem<T>::from_f(f[i]);
+    for (int i = 0; i < V / 2; ++i) {
+      const float2 x = f2_unpack(f[i]);
+      if constexpr (sizeof(T) == 4) {
+        w[2 * i] = __float_as_uint(x.x);
+        w[2 * i + 1] = __float_as_uint(x.y);
+      } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x.x, x.y);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      } else {
+        const __half2 h = __floats2half2_rn(x.x, x.y);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    }
   }
 };
 
-template <int V>
-__device__ __forceinline__ void load_floats(const float* p, float (&f)[V]) {
+// N floats from a 16-byte boundary (the vector kernels take tables whose rows and halves start on one)
+// as packed pairs.
+template <int N, int P>
+__device__ __forceinline__ void load_floats(const float* p, uint64_t (&f)[P]) {
+  static_assert(N % 2 == 0 && N <= 2 * P, "");
+  if constexpr (N % 4 == 0) {
 #pragma unroll
-  for (int i = 0; i < V; i += 2) {   // 8-byte aligned: the table's rows have an even number of floats
-    const float2 x = __ldg(reinterpret_cast<const float2*>(p + i));
-    f[i] = x.x; f[i + 1] = x.y;
+    for (int i = 0; i < N; i += 4) {
+      const float4 x = __ldg(reinterpret_cast<const float4*>(p + i));
+      f[i / 2] = f2_pack(x.x, x.y);
+      f[i / 2 + 1] = f2_pack(x.z, x.w);
+    }
+  } else {
+    const float2 x = __ldg(reinterpret_cast<const float2*>(p));
+    f[0] = f2_pack(x.x, x.y);
   }
 }
 
-template <int V>
-__device__ __forceinline__ void store_codes(uint8_t* p, const float (&f)[V], const Divisor& d) {
-  uint32_t c[V / 4];
+template <int P>
+__device__ __forceinline__ void store_codes(uint8_t* p, const uint64_t (&f)[P], const Divisor& d) {
+  uint32_t c[P / 2];
 #pragma unroll
-  for (int i = 0; i < V / 4; ++i)
-    c[i] = quant_e4m3x2(f[4 * i], f[4 * i + 1], d) | ((uint32_t)quant_e4m3x2(f[4 * i + 2], f[4 * i + 3], d) << 16);
-  if constexpr (V == 8) *reinterpret_cast<uint2*>(p) = make_uint2(c[0], c[1]);
+  for (int i = 0; i < P / 2; ++i) {
+    const float2 x = f2_unpack(f[2 * i]), y = f2_unpack(f[2 * i + 1]);
+    c[i] = quant_e4m3x2(x.x, x.y, d) | ((uint32_t)quant_e4m3x2(y.x, y.y, d) << 16);
+  }
+  if constexpr (P == 4) *reinterpret_cast<uint2*>(p) = make_uint2(c[0], c[1]);
   else *reinterpret_cast<uint32_t*>(p) = c[0];
 }
 
 // A team of `lanes` lanes (a power of two) serves HPT consecutive heads of one token, queries
 // first, then keys, then values.
 template <typename T, int V, int HPT>
-__global__ void __launch_bounds__(kRopeThreads) qk_rope_kernel(const __grid_constant__ RopeArgs a, int lanes, int pairs,
-                                                               int groups) {
+__global__ void __launch_bounds__(kRopeThreads, HPT == 1 ? 1 : kRopeBlocks) qk_rope_kernel(const __grid_constant__ RopeArgs a, int llanes, int pairs,
+                                                               uint32_t groups) {
   pdl_trigger();
   pdl_wait();            // launched as a programmatic dependent: global data from here on
-  const int64_t team = ((int64_t)blockIdx.x * kRopeThreads + threadIdx.x) / lanes;
+  const int lanes = 1 << llanes;
+  const uint32_t team = blockIdx.x * (kRopeThreads >> llanes) + (threadIdx.x >> llanes);   // below 2^32: the host checks
   const int li = threadIdx.x & (lanes - 1);
-  const int64_t tok = team / groups;
+  const uint32_t tok32 = team / groups;
+  const int64_t tok = tok32;
   if (tok >= a.tokens) return;   // whole teams leave; the shuffles below name the team's own lanes
-  const int h0 = (int)(team - tok * groups) * HPT;
+  const int h0 = (int)(team - tok32 * groups) * HPT;
   const uint32_t mask = (lanes == 32 ? 0xffffffffu : ((1u << lanes) - 1u)) << ((threadIdx.x & 31) & ~(lanes - 1));
   const int heads = a.hq + a.hkv + (a.v ? a.hkv : 0);
   const int half = a.R >> 1;
@@ -150,8 +189,8 @@ __global__ void __launch_bounds__(kRopeThreads) qk_rope_kernel(const __grid_cons
     if (h < a.hq) src = reinterpret_cast<const T*>(a.q) + tok * a.q_ts + h * a.q_hs;
     else if (h < a.hq + a.hkv) src = reinterpret_cast<const T*>(a.k) + tok * a.k_ts + (h - a.hq) * a.k_hs;
     else src = reinterpret_cast<const T*>(a.v) + tok * a.v_ts + (h - a.hq - a.hkv) * a.v_hs;
-    if (has_a) xa[i].load(src + ea);
-    if (has_b) xb[i].load(src + eb);
+    if (has_a) xa[i].template load<true>(src + ea);
+    if (has_b) xb[i].template load<true>(src + eb);
   }
   const int64_t pos = load_index(a.positions, a.pos64, tok);
   const bool pos_ok = pos >= 0 && pos < a.max_pos;
@@ -166,11 +205,12 @@ __global__ void __launch_bounds__(kRopeThreads) qk_rope_kernel(const __grid_cons
   if (!pos_ok && li == 0) atomicOr(&g_tu_status, kStatusBadRopeIndex);
 
   // cos / sin: V values each; interleaved, the first half belongs to xa and the second to xb
-  float c[V], s[V];
+  constexpr int P = V / 2;
+  uint64_t c[P], s[P];
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    c[i] = 1.0f;
-    s[i] = 0.0f;
+  for (int i = 0; i < P; ++i) {
+    c[i] = f2_pack(1.0f, 1.0f);
+    s[i] = 0ull;
   }
   if (pos_ok && active && h0 < a.hq + a.hkv) {
     const float* row = a.cos_sin + pos * a.R;
@@ -179,20 +219,19 @@ __global__ void __launch_bounds__(kRopeThreads) qk_rope_kernel(const __grid_cons
         load_floats<V>(row + ea, c);
         load_floats<V>(row + half + ea, s);
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const int e = i < V / 2 ? ea + 2 * i : eb + 2 * (i - V / 2);   // first element of the pair
-        if (e < a.R) {
-          c[i] = __ldg(row + (e >> 1));
-          s[i] = __ldg(row + half + (e >> 1));
-        }
-      }
+    } else if (rot_b) {                      // the lane's pairs are V consecutive ones
+      load_floats<V>(row + (ea >> 1), c);
+      load_floats<V>(row + half + (ea >> 1), s);
+    } else if (rot_a) {
+      load_floats<V / 2>(row + (ea >> 1), c);
+      load_floats<V / 2>(row + half + (ea >> 1), s);
     }
   }
   int64_t koff = 0, voff = 0;
   if (slot >= 0) {
-    const int64_t blk = slot / a.bs, in = slot - blk * a.bs;
+    // 32-bit division where the slots allow it
+    const int64_t blk = a.num_slots <= 0xffffffffLL ? (int64_t)((uint32_t)slot / (uint32_t)a.bs) : slot / a.bs;
+    const int64_t in = slot - blk * a.bs;
     koff = blk * a.k_bs + in * a.hkv * (int64_t)a.D;
     voff = blk * a.v_bs + in * a.hkv * (int64_t)a.D;
   }
@@ -201,9 +240,9 @@ __global__ void __launch_bounds__(kRopeThreads) qk_rope_kernel(const __grid_cons
   for (int i = 0; i < HPT; ++i) {
     const int h = h0 + i;
     if (h >= heads) break;
-    float fa[V], fb[V];
+    uint64_t fa[P], fb[P];
 #pragma unroll
-    for (int e = 0; e < V; ++e) fa[e] = fb[e] = 0.0f;
+    for (int e = 0; e < P; ++e) fa[e] = fb[e] = 0ull;
     if (has_a) xa[i].unpack(fa);
     if (has_b) xb[i].unpack(fb);
     const bool is_v = h >= a.hq + a.hkv;
@@ -211,47 +250,54 @@ __global__ void __launch_bounds__(kRopeThreads) qk_rope_kernel(const __grid_cons
     if (!is_v) {
       const T* w = reinterpret_cast<const T*>(is_k ? a.k_weight : a.q_weight);
       if (w) {
-        float ss = 0.0f;
+        uint64_t s2 = 0ull;
 #pragma unroll
-        for (int e = 0; e < V; ++e) ss += fa[e] * fa[e] + fb[e] * fb[e];
+        for (int e = 0; e < P; ++e) s2 = f2_fma(fb[e], fb[e], f2_fma(fa[e], fa[e], s2));
+        const float2 sq = f2_unpack(s2);
+        float ss = sq.x + sq.y;
         for (int o = lanes >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
         const float r = rsqrtf(ss / (float)a.D + a.eps);
+        const uint64_t r2 = f2_pack(r, r);
         VecN<T, V> wv;
-        float wf[V];
+        uint64_t wf[P];
         if (has_a) {
           wv.load(w + ea);
           wv.unpack(wf);
 #pragma unroll
-          for (int e = 0; e < V; ++e) fa[e] = fa[e] * r * wf[e];
+          for (int e = 0; e < P; ++e) fa[e] = f2_mul(f2_mul(fa[e], r2), wf[e]);
         }
         if (has_b) {
           wv.load(w + eb);
           wv.unpack(wf);
 #pragma unroll
-          for (int e = 0; e < V; ++e) fb[e] = fb[e] * r * wf[e];
+          for (int e = 0; e < P; ++e) fb[e] = f2_mul(f2_mul(fb[e], r2), wf[e]);
         }
       }
       if (!a.interleaved) {
+        const uint64_t minus = f2_pack(-1.0f, -1.0f);
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const float y = fa[e], z = fb[e];
-          fa[e] = y * c[e] - z * s[e];
-          fb[e] = z * c[e] + y * s[e];
+        for (int e = 0; e < P; ++e) {
+          const uint64_t y = fa[e], z = fb[e];
+          fa[e] = f2_fma(y, c[e], f2_mul(f2_mul(z, s[e]), minus));
+          fb[e] = f2_fma(z, c[e], f2_mul(y, s[e]));
         }
       } else {
+        // (y, z) -> (y, z) c + (-z, y) s; pair e of the lane has component e of c and s
+        auto turn = [&](uint64_t yz, int e) -> uint64_t {
+          const float2 v = f2_unpack(yz), c2 = f2_unpack(c[e >> 1]), s2 = f2_unpack(s[e >> 1]);
+          const float ce = e & 1 ? c2.y : c2.x, se = e & 1 ? s2.y : s2.x;
+          return f2_fma(yz, f2_pack(ce, ce), f2_mul(f2_pack(-v.y, v.x), f2_pack(se, se)));
+        };
 #pragma unroll
-        for (int e = 0; e < V / 2; ++e) {
-          const float y = fa[2 * e], z = fa[2 * e + 1];
-          fa[2 * e] = y * c[e] - z * s[e];
-          fa[2 * e + 1] = z * c[e] + y * s[e];
-          const float u = fb[2 * e], t = fb[2 * e + 1];
-          fb[2 * e] = u * c[V / 2 + e] - t * s[V / 2 + e];
-          fb[2 * e + 1] = t * c[V / 2 + e] + u * s[V / 2 + e];
+        for (int e = 0; e < P; ++e) {
+          fa[e] = turn(fa[e], e);
+          fb[e] = turn(fb[e], P + e);
         }
       }
       if (!pos_ok) {
+        const float nan = __int_as_float(0x7fc00000);
 #pragma unroll
-        for (int e = 0; e < V; ++e) fa[e] = fb[e] = __int_as_float(0x7fc00000);
+        for (int e = 0; e < P; ++e) fa[e] = fb[e] = f2_pack(nan, nan);
       }
     }
     VecN<T, V> o;
@@ -269,8 +315,8 @@ __global__ void __launch_bounds__(kRopeThreads) qk_rope_kernel(const __grid_cons
       if (a.e4m3) {
         uint8_t* dst = reinterpret_cast<uint8_t*>(is_v ? a.v_out : a.k_out) + off;
         const Divisor d = make_divisor(__ldg((is_v ? a.v_scale : a.k_scale) + kh));
-        if (has_a) store_codes<V>(dst + ea, fa, d);
-        if (has_b) store_codes<V>(dst + eb, fb, d);
+        if (has_a) store_codes(dst + ea, fa, d);
+        if (has_b) store_codes(dst + eb, fb, d);
       } else {
         T* dst = reinterpret_cast<T*>(is_v ? a.v_out : a.k_out) + off;
         if (has_a) { o.pack(fa); o.store(dst + ea); }
@@ -365,16 +411,18 @@ template <typename T, int V>
 cudaError_t launch_rope(const RopeArgs& a, cudaStream_t st) {
   const int heads = a.hq + a.hkv + (a.v ? a.hkv : 0);
   const int pairs = a.interleaved ? (a.D + 2 * V - 1) / (2 * V) : a.R / (2 * V) + (a.D - a.R + 2 * V - 1) / (2 * V);
-  int lanes = 1;
-  while (lanes < pairs) lanes <<= 1;
-  // Four heads a team once that still gives every SM several blocks: cos and sin are then loaded
-  // once for four heads and eight vector loads are in flight per lane.
-  const bool four = a.tokens * ((heads + 3) / 4) * lanes >= 148LL * 4 * kRopeThreads;
-  const int groups = four ? (heads + 3) / 4 : heads;
-  const int64_t blocks = (a.tokens * groups * lanes + kRopeThreads - 1) / kRopeThreads;
-  if (blocks > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
-  if (four) return launch_pdl(qk_rope_kernel<T, V, 4>, dim3((unsigned)blocks), dim3(kRopeThreads), 0, st, a, lanes, pairs, groups);
-  return launch_pdl(qk_rope_kernel<T, V, 1>, dim3((unsigned)blocks), dim3(kRopeThreads), 0, st, a, lanes, pairs, groups);
+  int llanes = 0;
+  while ((1 << llanes) < pairs) ++llanes;
+  // Two heads a team once that still gives every SM its blocks: cos and sin are then loaded once for both
+  // and four vector loads are in flight per lane (8192 tokens of 32 + 8 heads of 128, bf16, normalised:
+  // 48.5 us; one head 55.7, four 55.8).
+  const int64_t per = kRopeThreads >> llanes;
+  const bool many = a.tokens * ((heads + kRopeHeads - 1) / kRopeHeads) >= 148LL * kRopeBlocks * per;
+  const int64_t groups = many ? (heads + kRopeHeads - 1) / kRopeHeads : heads;
+  const int64_t blocks = (a.tokens * groups + per - 1) / per;
+  if (blocks > 0x7fffffffLL || blocks * per > 0xffffffffLL) return cudaErrorInvalidConfiguration;
+  if (many) return launch_pdl(qk_rope_kernel<T, V, kRopeHeads>, dim3((unsigned)blocks), dim3(kRopeThreads), 0, st, a, llanes, pairs, (uint32_t)groups);
+  return launch_pdl(qk_rope_kernel<T, V, 1>, dim3((unsigned)blocks), dim3(kRopeThreads), 0, st, a, llanes, pairs, (uint32_t)groups);
 }
 
 template <typename T>
@@ -406,7 +454,9 @@ int run_rope(const char* what, RopeArgs& a, int dtype, cudaStream_t st) {
     auto on = [&](const void* p) { return (reinterpret_cast<uintptr_t>(p) & (ab - 1)) == 0; };
     auto even = [&](int64_t s) { return (s * es) % (int64_t)ab == 0; };
     const int64_t cache_al = a.e4m3 ? v : (int64_t)ab / es;      // elements
-    const bool ok = a.D % v == 0 && a.R % unit == 0 && a.D <= 64 * v && on(a.q) && on(a.k) && on(a.q_out) &&
+    // cos and sin: rows and their halves on 16 bytes (interleaved V = 4: 8 bytes do, but one rule serves)
+    const bool table = (reinterpret_cast<uintptr_t>(a.cos_sin) & 15) == 0 && a.R % 8 == 0;
+    const bool ok = table && a.D % v == 0 && a.R % unit == 0 && a.D <= 64 * v && on(a.q) && on(a.k) && on(a.q_out) &&
                     (!a.q_weight || on(a.q_weight)) && (!a.k_weight || on(a.k_weight)) && even(a.q_ts) && even(a.q_hs) &&
                     even(a.k_ts) && even(a.k_hs) &&
                     (a.v ? on(a.v) && even(a.v_ts) && even(a.v_hs) && a.k_bs % cache_al == 0 && a.v_bs % cache_al == 0 &&
