@@ -445,7 +445,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
       }
       if constexpr (kE4m3) {
         const uint32_t pitch = ((uint32_t)(box * D) + 127u) & ~127u;
-        const int chunks = D / 16, lbox = __ffs(box) - 1;       // 16 codes a chunk
+        const int lbox = __ffs(box) - 1;
         for (int i = 0; i < 2 * g.T && ok; ++i, ++u) {
           const uint32_t sr = u % NR, s = u % NS;
           if (!warp_wait(&raw_full[sr], (u / NR) & 1)) s_abort = 1;
@@ -458,24 +458,30 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
           const uint8_t* raw = smem + L::kRaw0 + sr * L::kRaw;
           uint8_t* dst = smem + L::kKv0 + s * L::kOp;
           const int end = it.r.kl - (g.kt0 + (i >> 1)) * kKeys;  // rows from here on are past the last token
-          // thread: chunk ht % (4 DC) of rows ht / (4 DC), + 128 / (4 DC), ...; the lanes of the second 64-element
-          // chunk store their halves in the other order, so a quarter-warp's stores cover all banks
-          constexpr int CPR = 4 * DC;
-          const int c = ht % CPR;
-          const uint32_t flip = (uint32_t)(c >> 2) & 1u;
-          if (c < chunks) {
-#pragma unroll 8
-            for (int r = ht / CPR; r < kKeys; r += kHelpers / CPR) {
-              uint4 x = *reinterpret_cast<const uint4*>(raw + (r >> lbox) * pitch + (r & (box - 1)) * D + c * 16);
-              if (r >= end) x = make_uint4(0u, 0u, 0u, 0u);
-              const uint4 lo = make_uint4(e4m3x2_to_f16x2(x.x), e4m3x2_to_f16x2(x.x >> 16), e4m3x2_to_f16x2(x.y),
-                                          e4m3x2_to_f16x2(x.y >> 16));
-              const uint4 hi = make_uint4(e4m3x2_to_f16x2(x.z), e4m3x2_to_f16x2(x.z >> 16), e4m3x2_to_f16x2(x.w),
-                                          e4m3x2_to_f16x2(x.w >> 16));
-              uint8_t* d = dst + (c >> 2) * kChunkBytes + r * 128;
-              const uint32_t q = ((2 * c) & 7) + flip;
-              *reinterpret_cast<uint4*>(d + ((q ^ (r & 7)) << 4)) = flip ? hi : lo;
-              *reinterpret_cast<uint4*>(d + (((q ^ 1u) ^ (r & 7)) << 4)) = flip ? lo : hi;
+          // Thread: eight codes, one 16-byte unit of the operand, of rows r0, r0 + step, ...: a quarter-warp's
+          // stores cover a row's eight units, and the swizzle (r & 7) is the thread's own.
+          constexpr int UPR = 8 * DC, step = kHelpers / UPR;      // units a row, rows a pass (a multiple of 8)
+          const int q = ht % UPR, r0 = ht / UPR;
+          uint8_t* const d0 = dst + (q >> 3) * kChunkBytes + r0 * 128 + (((q & 7) ^ (r0 & 7)) << 4);
+          auto put = [&](uint8_t* d, uint2 x) {
+            *reinterpret_cast<uint4*>(d) =
+                make_uint4(e4m3x2_to_f16x2(x.x), e4m3x2_to_f16x2(x.x >> 16), e4m3x2_to_f16x2(x.y), e4m3x2_to_f16x2(x.y >> 16));
+          };
+          if (D == 64 * DC && end >= kKeys) {                     // whole tiles of whole chunks: rows one after another
+            const uint8_t* const r8 = raw + r0 * (64 * DC) + q * 8;
+#pragma unroll
+            for (int k = 0; k < kKeys / step; k += 8) {
+              uint2 x[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) x[e] = *reinterpret_cast<const uint2*>(r8 + (k + e) * step * 64 * DC);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) put(d0 + (k + e) * step * 128, x[e]);
+            }
+          } else if (q * 8 < D) {
+            for (int r = r0; r < kKeys; r += step) {
+              uint2 x = make_uint2(0u, 0u);
+              if (r < end) x = *reinterpret_cast<const uint2*>(raw + (r >> lbox) * pitch + (r & (box - 1)) * D + q * 8);
+              put(d0 + (r - r0) * 128, x);
             }
           }
           fence_async_smem();
