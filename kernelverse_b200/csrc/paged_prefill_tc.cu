@@ -47,7 +47,7 @@ constexpr int kHalf = 64;                  // keys whose P is handed over at a t
 constexpr int kTile = 2 * kRows;           // rows of a tile
 constexpr int kThreads = 512;
 constexpr int kHelpers = 128;              // threads of warps 12-15
-constexpr int kSoftmaxRegs = 192, kOtherRegs = 64;   // 2 x 128 x (192 + 64) = 512 x 128: what the block is launched with
+constexpr int kSoftmaxRegs = 176, kOtherRegs = 80;   // 2 x 128 x (176 + 80) = 512 x 128: what the block is launched with
 constexpr int kMaxSlots = 8;
 constexpr int kMaxRaw = 4;
 
