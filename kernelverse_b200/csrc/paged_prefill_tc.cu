@@ -4,22 +4,20 @@
 //
 // One persistent CTA per SM works through its share of (request, KV head, row tile) items
 // (paged_prefill.cuh).  The query rows of a KV head's group are packed (row = token x group + head), so
-// each key is read once for the whole group.  Two chains S = Q K^T -> softmax -> O += P V run side by
-// side, each with 128 rows (TMEM lanes), an S buffer of 128 keys and its O in tensor memory and four
-// softmax warps, so one chain's exponentials overlap the other's products:
-//   wide items (over 128 rows): chain A has rows 0..127 of the tile, chain B rows 128..255, and both
-//     use every K/V tile of 128 keys;
+// each key is read once for the whole group.  Two chains run side by side, each with 128 rows (TMEM
+// lanes), four softmax warps, its O and two S buffers of 64 keys in tensor memory:
+//   S_n = Q K_n^T -> buffer n % 2;  softmax: P_n over S_n;  O += P_n V_n
+// with S_{n+1} computed while the softmax of S_n runs:
+//   wide items (over 128 rows): chain A has rows 0..127 of the tile, chain B rows 128..255; each goes
+//     through both 64-key halves of every K/V tile of 128 keys;
 //   deep items (at most 128 rows: decoding, drafts, the last rows of a prompt): both chains have the
-//     same rows, A takes the even K/V tiles and B the odd ones, and the two results are joined.
-// A chain hands P over in two halves, so the first half of PV runs under the second half's
-// exponentials.  (Two S buffers of 64 keys a chain instead, with the next S computed under the softmax,
-// measured the same: products with N = 64 take as long as with N = 128.)
+//     same rows, A takes the lower half of each K/V tile and B the upper one, and the two results are
+//     joined.
 // Roles: warp 0 issues the TMA loads (boxes of whole page runs gathered through the block table); one
 // lane each of warps 1 and 2 issues the MMAs of chain A and of chain B (one issuer for both was the
 // limit: its 16 MMAs, four commits and four waits a tile took ~2900 cycles, against 1024 of tensor
 // time); warp 3 zeroes page tails; warps 4-7 and 8-11 are the softmax groups of A and B; warps 12-15
-// gather the query rows and turn e4m3 codes into float16 operands.  The softmax warps take the registers
-// that the others give up, so a row's 128 scores stay in registers.
+// gather the query rows and turn e4m3 codes into float16 operands.
 // K and V tiles share one ring of shared-memory slots in the order K_0 V_0 K_1 V_1 ...  A page outside
 // the cache, and pages past the last token, are loaded from an out-of-range block coordinate, which
 // TMA fills with zeros; the rows past the last token inside its page are zeroed in shared memory.
@@ -43,11 +41,11 @@ namespace {
 
 constexpr int kRows = 128;                 // rows of a chain (TMEM lanes)
 constexpr int kKeys = 128;                 // keys per K/V tile
-constexpr int kHalf = 64;                  // keys whose P is handed over at a time
+constexpr int kHalf = 64;                  // keys of an S buffer
 constexpr int kTile = 2 * kRows;           // rows of a tile
 constexpr int kThreads = 512;
 constexpr int kHelpers = 128;              // threads of warps 12-15
-constexpr int kSoftmaxRegs = 176, kOtherRegs = 80;   // 2 x 128 x (176 + 80) = 512 x 128: what the block is launched with
+
 constexpr int kMaxSlots = 8;
 constexpr int kMaxRaw = 4;
 
@@ -77,42 +75,51 @@ __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two) {
   return r;
 }
 
-// What every role derives from an item: key tiles [kt0, kt0 + T), and which of them each chain uses.
+// What every role derives from an item: key tiles [kt0, kt0 + T) of 128 keys, and the 64-key halves that
+// each chain goes through.
 struct PcItem {
   int row0;        // first row of the tile in its request
   int rows;        // rows of the tile
   bool wide;
   int kt0, T;
   int TA;          // wide: how many of the tiles chain A uses
+  int subs_a, subs_b;   // halves of each chain
   __device__ __forceinline__ PcItem(const PagedArgs& a, const PgItem& it) {
     row0 = it.t * kTile;
     rows = min(kTile, it.r.ql * a.group - row0);
     wide = rows > kRows;
     kt0 = it.j0;
     T = it.j1 - it.j0;
-    const int xa = (it.r.kl - it.r.ql) * a.group + row0 + kRows - 1;       // position x group of chain A's last row
-    TA = max(1, min(T, (xa < 0 ? 0 : xa / (a.group * kKeys) + 1) - kt0));  // (a tile that it sees nothing of keeps the chains in step)
+    const int x0 = (it.r.kl - it.r.ql) * a.group + row0;        // position x group of the first row
+    const int xb = x0 + rows - 1;
+    const int seen = xb < 0 ? 0 : xb / a.group;                 // last key that the last row sees
+    const bool low = it.j1 * kKeys - kHalf > seen;              // the upper half of the last tile: nobody sees it
+    TA = T;
+    if (wide) {
+      const int xa = x0 + kRows - 1;
+      const int seen_a = xa < 0 ? 0 : xa / a.group;
+      TA = max(1, min(T, seen_a / kKeys + 1 - kt0));            // (a tile that it sees nothing of keeps the chains in step)
+      subs_a = 2 * TA - ((kt0 + TA) * kKeys - kHalf > seen_a ? 1 : 0);
+      subs_b = 2 * T - (low ? 1 : 0);
+    } else {
+      subs_a = T;
+      subs_b = T - (low ? 1 : 0);
+    }
   }
-  // tiles of chain c, and its k-th
-  __device__ __forceinline__ int count(int c) const { return wide ? (c ? T : TA) : (T - c + 1) >> 1; }
-  __device__ __forceinline__ int tile(int c, int k) const { return wide ? k : 2 * k + c; }
+  __device__ __forceinline__ int subs(int c) const { return c ? subs_b : subs_a; }
+  // tile (of the item) and half of the chain's m-th half
+  __device__ __forceinline__ int tile(int m) const { return wide ? m >> 1 : m; }
+  __device__ __forceinline__ int half(int c, int m) const { return wide ? m & 1 : c; }
+  // whether the chain is done with the tile after its m-th half
+  __device__ __forceinline__ bool leaves(int c, int m) const { return !wide || (m & 1) || m + 1 == subs(c); }
   // whether one chain alone uses tile i
-  __device__ __forceinline__ bool one_user(int i) const { return !wide || i >= TA; }
+  __device__ __forceinline__ bool one_user(int i) const { return wide ? i >= TA : i >= subs_b; }
 };
 // Rows of key tile kt past the last token that a box of the tile holds together with tokens.
 __device__ __forceinline__ int tail_rows(int kl, int kt, int box) {
   const int end = kl - kt * kKeys, in = end & (box - 1);
   return end > 0 && end < kKeys && in ? box - in : 0;
 }
-
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
-
-template <int N> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
-template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 
 template <typename T, bool kE4m3, int DC>
 __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __grid_constant__ CUtensorMap tk,
@@ -129,7 +136,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
   const uint32_t sbase = smem_u32(smem);
   __shared__ uint64_t kv_full[kMaxSlots], kv_empty[kMaxSlots], tail_full[kE4m3 ? 1 : kMaxSlots],
       raw_full[kE4m3 ? kMaxRaw : 1], raw_empty[kE4m3 ? kMaxRaw : 1],
-      q_full, q_empty, s_full[2], p_half[2], p_full[2], pv_done[2], mma_done[2], joined;
+      q_full, q_empty, s_full[4], p_full[4], pv_done[4], mma_done[2], joined;   // s, p, pv: [2 * chain + buffer]
   __shared__ uint32_t tmem_base_s;
   __shared__ volatile int s_abort;
   __shared__ PgShare share;
@@ -151,13 +158,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
     }
     mbar_init(&q_full, 4);
     mbar_init(&q_empty, 2);
-    for (int c = 0; c < 2; ++c) {
+    for (int c = 0; c < 4; ++c) {
       mbar_init(&s_full[c], 1);
-      mbar_init(&p_half[c], 4);
       mbar_init(&p_full[c], 4);
       mbar_init(&pv_done[c], 1);
-      mbar_init(&mma_done[c], 1);
     }
+    mbar_init(&mma_done[0], 1);
+    mbar_init(&mma_done[1], 1);
     mbar_init(&joined, 8);
     s_abort = 0;
     fence_mbar_init();
@@ -184,8 +191,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
   PgWalk walk(share);
   PgItem it;
 
-  if (warp < 4) {
-  regs_down<kOtherRegs>();
   if (warp == 0) {
     // ---------------------------------------------------------------- TMA producer
     // A tile is kKeys / box boxes of `box` keys, each inside one page; lane l serves box l % boxes.
@@ -263,78 +268,65 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
     {
       const int c = warp - 1;
       const uint32_t tb = tmem + (uint32_t)c * 256u;
-      constexpr uint32_t kIdS = idesc_f16(kRows, kKeys, kBf, false);
+      constexpr uint32_t kIdS = idesc_f16(kRows, kHalf, kBf, false);
       const uint32_t id_pv = idesc_f16(kRows, D, kBf, true);
       uint32_t u0 = 0, item = 0;                               // ring position of the item's first tile
-      uint32_t n = 0;                                          // tiles of the chain so far, all items
+      uint32_t n = 0;                                          // halves of the chain whose S has been issued, all items
       bool ok = true;
       while (ok && walk.next(a, tiles, it)) {
         const PcItem g(a, it);
-        const int count = g.count(c);
+        const int subs = g.subs(c);
         const uint64_t qd = desc_kmajor(sbase + L::kQ0 + (g.wide ? c : 0) * L::kOp);
-        auto wait_k = [&](int k) -> bool {
-          const uint32_t v = u0 + 2 * g.tile(c, k);
-          return warp_wait(&kv_full[v % NS], (v / NS) & 1);
-        };
-        auto issue_s = [&](int k) {                            // K has landed, the P that S overwrites is used up
-          const uint32_t s = (u0 + 2 * g.tile(c, k)) % NS;
+        auto issue_s = [&](int m) -> bool {
+          const uint32_t v = u0 + 2 * g.tile(m), s = v % NS, b = n & 1;
+          if (!warp_wait(&kv_full[s], (v / NS) & 1)) return false;
+          if (n > 1 && !warp_wait(&pv_done[2 * c + b], ((n >> 1) - 1) & 1)) return false;   // the P it overwrites is used up
           tc_fence_after();
-          const uint64_t kd = desc_kmajor(sbase + L::kKv0 + s * L::kOp);
+          const uint64_t kd = desc_kmajor(sbase + L::kKv0 + s * L::kOp) + g.half(c, m) * (kHalf * 128 >> 4);
+          const bool leaves = g.leaves(c, m), last = m + 1 == subs;
           if (elect_one()) {
-          // 16 elements = 32 bytes on in both operands, 64 elements one chunk on
-          if (D == 64 * DC) {
+            // 16 elements = 32 bytes on in both operands, 64 elements one chunk on
+            if (D == 64 * DC) {
 #pragma unroll
-            for (int ks = 0; ks < 4 * DC; ++ks)
-              mma_f16(tb, qd + (ks >> 2) * (kChunkBytes >> 4) + (ks & 3) * 2, kd + (ks >> 2) * (kChunkBytes >> 4) + (ks & 3) * 2,
-                      kIdS, ks > 0);
-          } else {
-            for (int ks = 0; ks < D / 16; ++ks)
-              mma_f16(tb, qd + (ks >> 2) * (kChunkBytes >> 4) + (ks & 3) * 2, kd + (ks >> 2) * (kChunkBytes >> 4) + (ks & 3) * 2,
-                      kIdS, ks > 0);
-          }
-          mma_commit(&s_full[c]);
-          mma_commit(&kv_empty[s]);
-          if (k + 1 == count) mma_commit(&q_empty);
+              for (int ks = 0; ks < 4 * DC; ++ks)
+                mma_f16(tb + b * kHalf, qd + (ks >> 2) * (kChunkBytes >> 4) + (ks & 3) * 2,
+                        kd + (ks >> 2) * (kChunkBytes >> 4) + (ks & 3) * 2, kIdS, ks > 0);
+            } else {
+              for (int ks = 0; ks < D / 16; ++ks)
+                mma_f16(tb + b * kHalf, qd + (ks >> 2) * (kChunkBytes >> 4) + (ks & 3) * 2,
+                        kd + (ks >> 2) * (kChunkBytes >> 4) + (ks & 3) * 2, kIdS, ks > 0);
+            }
+            mma_commit(&s_full[2 * c + b]);
+            if (leaves) mma_commit(&kv_empty[s]);
+            if (last) mma_commit(&q_empty);
           }
           __syncwarp();
+          ++n;
+          return true;
         };
         ok = warp_wait(&q_full, item & 1);
         ++item;
-        if (count == 0 && ok && lane == 0) mbar_arrive(&q_empty);
-        if (count > 0) {
-          ok = ok && wait_k(0) && (n == 0 || warp_wait(&pv_done[c], (n - 1) & 1));
-          if (ok) issue_s(0);
-        }
-        for (int k = 0; k < count && ok; ++k, ++n) {
-          const uint32_t v = u0 + 2 * g.tile(c, k) + 1, s = v % NS;
-          ok = warp_wait(&kv_full[s], (v / NS) & 1);
-          // (in a deep item the next K may want the slot of this very V: it is waited for after PV)
-          if (ok && g.wide && k + 1 < count) ok = wait_k(k + 1);
-          ok = ok && warp_wait(&p_half[c], n & 1);
+        if (subs == 0 && ok && lane == 0) mbar_arrive(&q_empty);
+        const uint32_t n0 = n;
+        if (subs > 0) ok = ok && issue_s(0);
+        if (subs > 1) ok = ok && issue_s(1);
+        for (int m = 0; m < subs && ok; ++m) {
+          const uint32_t v = u0 + 2 * g.tile(m) + 1, s = v % NS, b = (n0 + m) & 1;
+          ok = warp_wait(&kv_full[s], (v / NS) & 1) && warp_wait(&p_full[2 * c + b], ((n0 + m) >> 1) & 1);
           if (!ok) break;
           tc_fence_after();
-          // 16 keys: 8 packed columns of P over the scores, 16 rows of V
-          const uint64_t vd = desc_mnmajor(sbase + L::kKv0 + s * L::kOp, kChunkBytes);
+          // 16 keys: 8 packed columns of P, 16 rows of V
+          const uint64_t vd = desc_mnmajor(sbase + L::kKv0 + s * L::kOp, kChunkBytes) + g.half(c, m) * (kHalf * 128 >> 4);
+          const bool leaves = g.leaves(c, m);
           if (elect_one()) {
 #pragma unroll
-            for (int ks = 0; ks < kHalf / 16; ++ks) mma_f16_ts(tb + 128u, tb + (uint32_t)ks * 8u, vd + ks * 128, id_pv, (k | ks) != 0);
+            for (int ks = 0; ks < kHalf / 16; ++ks)
+              mma_f16_ts(tb + 128u, tb + b * kHalf + (uint32_t)ks * 8u, vd + ks * 128, id_pv, (m | ks) != 0);
+            mma_commit(&pv_done[2 * c + b]);
+            if (leaves) mma_commit(&kv_empty[s]);
           }
           __syncwarp();
-          ok = warp_wait(&p_full[c], n & 1);
-          if (!ok) break;
-          tc_fence_after();
-          if (elect_one()) {
-#pragma unroll
-            for (int ks = kHalf / 16; ks < kKeys / 16; ++ks) mma_f16_ts(tb + 128u, tb + (uint32_t)ks * 8u, vd + ks * 128, id_pv, 1);
-            mma_commit(&pv_done[c]);
-            mma_commit(&kv_empty[s]);
-          }
-          __syncwarp();
-          if (k + 1 < count) {
-            if (!g.wide) ok = wait_k(k + 1);
-            ok = ok && warp_wait(&pv_done[c], n & 1);
-            if (ok) issue_s(k + 1);
-          }
+          if (m + 2 < subs) ok = issue_s(m + 2);
         }
         u0 += 2 * g.T;
         if (__any_sync(0xffffffffu, s_abort)) ok = false;
@@ -372,9 +364,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
         if (__any_sync(0xffffffffu, s_abort)) ok = false;
       }
     }
-  }
   } else if (warp >= 12) {
-    regs_down<kOtherRegs>();
     // ---------------------------------------------------------------- helpers: query rows, e4m3 codes to float16
     const int ht = threadIdx.x - 384;                                     // 0 .. 127
     uint32_t u = 0, item = 0;
@@ -494,14 +484,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
       }
     }
   } else {
-    regs_up<kSoftmaxRegs>();
     // ---------------------------------------------------------------- softmax (warps 4-7: chain A, 8-11: chain B)
     const int c = (warp - 4) >> 2;
     const int quarter = warp & 3;                          // TMEM lanes this warp may access
     const int row = quarter * 32 + lane;                   // row of the chain = TMEM lane
     const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
     const uint32_t s_col = tmem + lane_addr + (uint32_t)c * 256u, o_col = s_col + 128u;
-    uint32_t n = 0, item = 0;                              // tiles of the chain so far; items
+    uint32_t n = 0, item = 0;                              // halves of the chain so far; items
     int64_t at = walk.at;                                  // first unit of the item's part
     uint32_t joins = 0;
     bool ok = true;
@@ -525,7 +514,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
       const int pos = valid ? off + tok : it.r.kl - 1;     // rows past the request compute on zeros, unseen
       const int pos_min = off + (g.row0 + (g.wide ? c * kRows : 0) + quarter * 32) / a.group;
       float sc = a.scale_log2;
-      const int nt = g.count(c);
+      const int nt = g.subs(c);
       if constexpr (kE4m3) {
         if (nt > 0) {
           if (!warp_wait(&q_full, item & 1)) s_abort = 1;
@@ -537,43 +526,42 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
       const uint64_t sc2 = f2_pack(sc, sc);
       float m = -INFINITY, l = 0.0f;                       // l: the sum of the P so far, at the scale 2^-m
       for (int i = 0; i < nt; ++i, ++n) {
-        if (!warp_wait(&s_full[c], n & 1)) {               // warp-uniform
+        const uint32_t b = n & 1, s_buf = s_col + b * kHalf;
+        if (!warp_wait(&s_full[2 * c + b], (n >> 1) & 1)) {   // warp-uniform
           ok = false;
           break;
         }
         tc_fence_after();
         if (any_valid) {
-          const int kb = (g.kt0 + g.tile(c, i)) * kKeys;
-          uint32_t r[2][kHalf];
-          tmem_ld64_async(s_col, r[0]);
-          tmem_ld64_async(s_col + kHalf, r[1]);
-          tmem_ld_wait(r[0]);
-          tmem_ld_wait(r[1]);
-          if (kb + kKeys - 1 > pos_min) {                  // some key of the tile may pass a row
+          const int kb = (g.kt0 + g.tile(i)) * kKeys + g.half(c, i) * kHalf;
+          uint32_t r[kHalf], w[kHalf / 2];
+          tmem_ld64_async(s_buf, r);
+          tmem_ld_wait(r);
+          if (kb + kHalf - 1 > pos_min) {                  // some key of the half may pass a row
 #pragma unroll
-            for (int e = 0; e < kKeys; ++e)
-              if (kb + e > pos) r[e >> 6][e & 63] = __float_as_uint(hidden);
+            for (int e = 0; e < kHalf; ++e)
+              if (kb + e > pos) r[e] = __float_as_uint(hidden);
           }
+          // (two-operand maxima: the three-operand ones took 160 cycles more per 128 scores)
           float x4[4] = {hidden, hidden, hidden, hidden};
           if (sc >= 0.0f) {
 #pragma unroll
-            for (int e = 0; e < kKeys; e += 2)
-              x4[(e >> 1) & 3] = max3(x4[(e >> 1) & 3], __uint_as_float(r[e >> 6][e & 63]), __uint_as_float(r[e >> 6][(e & 63) + 1]));
+            for (int e = 0; e < kHalf; ++e) x4[e & 3] = fmaxf(x4[e & 3], __uint_as_float(r[e]));
           } else {
 #pragma unroll
-            for (int e = 0; e < kKeys; ++e) x4[e & 3] = fminf(x4[e & 3], __uint_as_float(r[e >> 6][e & 63]));
+            for (int e = 0; e < kHalf; ++e) x4[e & 3] = fminf(x4[e & 3], __uint_as_float(r[e]));
           }
-          const float ext = sc >= 0.0f ? max3(fmaxf(x4[0], x4[1]), x4[2], x4[3]) : fminf(fminf(x4[0], x4[1]), fminf(x4[2], x4[3]));
+          const float ext = sc >= 0.0f ? fmaxf(fmaxf(x4[0], x4[1]), fmaxf(x4[2], x4[3])) : fminf(fminf(x4[0], x4[1]), fminf(x4[2], x4[3]));
           const float mx = ext * sc - kUp;                 // log2 domain; -inf where the row sees nothing
           // The maximum only moves when it grows by more than 2^8: sum and O carry the same factor, so the
-          // result is unchanged, and most tiles need no rescaling.
+          // result is unchanged, and most halves need no rescaling.
           const bool grow = mx > m + kGrow;
           if (__any_sync(0xffffffffu, grow)) {
             const float alpha = grow ? ex2_approx(m - mx) : 1.0f;
             if (grow) m = mx;
             l *= alpha;
             if (i > 0) {                                   // O *= alpha, once the chain's last PV has completed
-              if (!warp_wait(&pv_done[c], (n - 1) & 1)) {
+              if (!warp_wait(&pv_done[2 * c + (b ^ 1)], ((n - 1) >> 1) & 1)) {
                 ok = false;
                 break;
               }
@@ -591,32 +579,21 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
           const uint64_t nm2 = f2_pack(neg_m, neg_m);
           uint64_t l2[2] = {0ull, 0ull};
 #pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
-            uint32_t w[kHalf / 2];
-#pragma unroll
-            for (int e = 0; e < kHalf; e += 2) {
-              const float2 x = f2_unpack(f2_fma(f2_pack(__uint_as_float(r[hf][e]), __uint_as_float(r[hf][e + 1])), sc2, nm2));
-              const float p0 = ex2_approx(x.x), p1 = ex2_approx(x.y);
-              l2[(e >> 1) & 1] = f2_add(l2[(e >> 1) & 1], f2_pack(p0, p1));
-              w[e >> 1] = pack2h<kBf>(p0, p1);
-            }
-            tmem_st32(s_col + 32u * hf, w);
-            if (hf == 0) {
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&p_half[c]);
-            }
+          for (int e = 0; e < kHalf; e += 2) {
+            const float2 x = f2_unpack(f2_fma(f2_pack(__uint_as_float(r[e]), __uint_as_float(r[e + 1])), sc2, nm2));
+            const float p0 = ex2_approx(x.x), p1 = ex2_approx(x.y);
+            l2[(e >> 1) & 1] = f2_add(l2[(e >> 1) & 1], f2_pack(p0, p1));
+            w[e >> 1] = pack2h<kBf>(p0, p1);
           }
+          tmem_st32(s_buf, w);
           const float2 ls = f2_unpack(f2_add(l2[0], l2[1]));
           l += ls.x + ls.y;
-        } else if (lane == 0) {
-          mbar_arrive(&p_half[c]);
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[c]);
+        if (lane == 0) mbar_arrive(&p_full[2 * c + b]);
       }
-      if (ok && nt > 0) ok = warp_wait(&pv_done[c], (n - 1) & 1);
+      if (ok && nt > 0) ok = warp_wait(&pv_done[2 * c + ((n - 1) & 1)], ((n - 1) >> 1) & 1);
       tc_fence_after();
       if (!ok) s_abort = 1;
       // ---- the item's result: finished, or a part of it
@@ -636,7 +613,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
         w_other = ex2_approx(m2 - mu);
         l = l * w_own + l2 * w_other;
         m = mj;
-        has_other = g.count(c ^ 1) > 0;
+        has_other = g.subs(c ^ 1) > 0;
       }
       if (ok && any_valid) {
         const float vsc = kE4m3 ? __ldg(a.v_scale + it.h) : 1.0f;
