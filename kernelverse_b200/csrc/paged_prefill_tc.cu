@@ -46,9 +46,6 @@ constexpr int kTile = 2 * kRows;           // rows of a tile
 constexpr int kThreads = 512;
 constexpr int kHelpers = 128;              // threads of warps 12-15
 
-constexpr int kMaxSlots = 8;
-constexpr int kMaxRaw = 4;
-
 template <bool kE4m3, int DC> struct PcLayout {
   static constexpr uint32_t kOp = DC * kChunkBytes;                // one Q, K or V tile of 16-bit operands
   static constexpr uint32_t kRaw = kE4m3 ? kKeys * 64u * DC : 0u;  // one K or V tile of codes
@@ -58,7 +55,7 @@ template <bool kE4m3, int DC> struct PcLayout {
   static constexpr int kSlots = kFit < 8 ? kFit : 8;
   static constexpr uint32_t kQ0 = 0, kKv0 = 2 * kOp, kRaw0 = kKv0 + kSlots * kOp;
   static constexpr size_t kSmem = kRaw0 + (size_t)kRawSlots * kRaw + 1024;
-  static_assert(kSlots >= 3 && kSlots <= kMaxSlots && kRawSlots <= kMaxRaw, "ring");
+  static_assert(kSlots >= 3, "ring");
 };
 
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
@@ -134,9 +131,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_u32(smem);
-  __shared__ uint64_t kv_full[kMaxSlots], kv_empty[kMaxSlots], tail_full[kE4m3 ? 1 : kMaxSlots],
-      raw_full[kE4m3 ? kMaxRaw : 1], raw_empty[kE4m3 ? kMaxRaw : 1],
-      q_full, q_empty, s_full[4], p_full[4], pv_done[4], mma_done[2], joined;   // s, p, pv: [2 * chain + buffer]
+  __shared__ uint64_t kv_full[NS], kv_empty[NS], tail_full[kE4m3 ? 1 : NS],
+      raw_full[kE4m3 ? NR : 1], raw_empty[kE4m3 ? NR : 1],
+      q_full, q_empty, s_full[4], p_full[4], pv_done[4], mma_done[2], joined,   // s, p, pv: [2 * chain + buffer]
+      sc_full[kE4m3 ? 2 : 1], q_seen[kE4m3 ? 2 : 1];   // an item's row scales are there, have been read: by item parity
   __shared__ uint32_t tmem_base_s;
   __shared__ volatile int s_abort;
   __shared__ PgShare share;
@@ -166,6 +164,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
     mbar_init(&mma_done[0], 1);
     mbar_init(&mma_done[1], 1);
     mbar_init(&joined, 8);
+    for (int x = 0; x < (kE4m3 ? 2 : 1); ++x) {
+      mbar_init(&sc_full[x], 4);
+      mbar_init(&q_seen[x], 8);
+    }
     s_abort = 0;
     fence_mbar_init();
     asm volatile("prefetch.tensormap [%0];" ::"l"(&tk) : "memory");
@@ -372,6 +374,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
     while (ok && walk.next(a, tiles, it)) {
       const PcItem g(a, it);
       if (item > 0 && !warp_wait(&q_empty, (item - 1) & 1)) s_abort = 1;
+      // S of a short item, and so q_empty, may be done while the softmax still is an item or two back: its row scales
+      // stay until it has read them (and have barriers of their own by item parity: a warp that is late cannot tell
+      // phase k of one barrier from phase k + 2)
+      if constexpr (kE4m3)
+        if (item > 1 && !warp_wait(&q_seen[item & 1], ((item >> 1) - 1) & 1)) s_abort = 1;
       if (__any_sync(0xffffffffu, s_abort)) break;
       {
         // Sixteen lanes (eight for D <= 64) take a row: eight elements each, whole rows coalesced.
@@ -430,7 +437,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
         }
         fence_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&q_full);
+        if (lane == 0) {
+          if constexpr (kE4m3) mbar_arrive(&sc_full[item & 1]);
+          mbar_arrive(&q_full);
+        }
         ++item;
       }
       if constexpr (kE4m3) {
@@ -516,10 +526,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
       float sc = a.scale_log2;
       const int nt = g.subs(c);
       if constexpr (kE4m3) {
-        if (nt > 0) {
-          if (!warp_wait(&q_full, item & 1)) s_abort = 1;
-          sc *= __ldg(a.k_scale + it.h) * __int_as_float((127 + (int)qexp_s[item & 1][trow]) << 23);
-        }
+        if (!warp_wait(&sc_full[item & 1], (item >> 1) & 1)) s_abort = 1;
+        sc *= __ldg(a.k_scale + it.h) * __int_as_float((127 + (int)qexp_s[item & 1][trow]) << 23);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&q_seen[item & 1]);
       }
       if (sc == 0.0f) sc = 1e-30f;                         // equal weights; a masked score stays -inf below
       const float hidden = sc >= 0.0f ? -INFINITY : INFINITY;

@@ -235,6 +235,17 @@ def test_many_requests():
     Case(15, chunks.tolist(), contexts.tolist(), 2, 1, 32, 16, "fp32").check(0)
 
 
+@pytest.mark.parametrize("tokens", [1, 2, 40])
+def test_many_short_requests_over_codes_keep_their_row_scales(tokens):
+    """Short items follow one another in a CTA faster than their softmax; each row has a scale of its own."""
+    rng = seeded(12 + tokens)
+    contexts = [int(c) for c in rng.integers(tokens, 140, 900)]
+    c = Case(11, [tokens] * 900, contexts, 8, 2, 128, 16, "bf16", "e4m3")
+    power = torch.from_numpy(rng.integers(-14, 3, c.q.shape[:2]).astype(np.float32)).cuda()
+    c.q = c.q * torch.exp2(power)[..., None].to(c.q.dtype)      # exact
+    c.check(2)
+
+
 def test_offsets_past_32_bits():
     """A cache of more than 2^31 elements whose pages lie at its end."""
     nb, bs, h, d = 17000, 16, 64, 128
