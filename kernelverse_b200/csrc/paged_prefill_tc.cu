@@ -10,10 +10,12 @@
 // with S_{n+1} computed while the softmax of S_n runs:
 //   wide items (over 128 rows): chain A has rows 0..127 of the tile, chain B rows 128..255; each goes
 //     through both 64-key halves of every K/V tile of 128 keys;
-//   deep items (at most 128 rows: decoding, drafts, the last rows of a prompt): both chains have the
-//     same rows, A takes the lower half of each K/V tile and B the upper one, and the two results are
-//     joined.
-// Roles: warp 0 issues the TMA loads (boxes of whole page runs gathered through the block table); one
+//   deep items (at most 128 rows: decoding, drafts, the last rows of a prompt): both chains have the same
+//     rows, A takes the lower half of each K/V tile and B the upper one, and the two results are joined;
+//   thin items (at most 16 rows over codes of head_dim 128: one decoded token's group, short drafts) go
+//     past the chains: thin_item below.
+// Roles: warp 0 issues the TMA loads (boxes of whole page runs gathered through the block table; over codes
+// warp 0 those of K and warp 3 those of V); one
 // lane each of warps 1 and 2 issues the MMAs of chain A and of chain B (one issuer for both was the
 // limit: its 16 MMAs, four commits and four waits a tile took ~2900 cycles, against 1024 of tensor
 // time); warp 3 zeroes page tails; warps 4-7 and 8-11 are the softmax groups of A and B; warps 12-15
@@ -28,11 +30,13 @@
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
+#include <cfloat>
 #include <mutex>
 #include <type_traits>
 
 #include "kvb_common.cuh"
 #include "kvb_async.cuh"
+#include "mma_sync.cuh"
 #include "paged_prefill.cuh"
 #include "tcgen05.cuh"
 
@@ -43,6 +47,7 @@ constexpr int kRows = 128;                 // rows of a chain (TMEM lanes)
 constexpr int kKeys = 128;                 // keys per K/V tile
 constexpr int kHalf = 64;                  // keys of an S buffer
 constexpr int kTile = 2 * kRows;           // rows of a tile
+constexpr int kThin = 16;                  // rows of a thin item at most
 constexpr int kThreads = 512;
 constexpr int kHelpers = 128;              // threads of warps 12-15
 
@@ -54,6 +59,7 @@ template <bool kE4m3, int DC> struct PcLayout {
   static constexpr int kFit = (int)((kBudget - 2 * kOp - kRawSlots * kRaw) / kOp);
   static constexpr int kSlots = kFit < 8 ? kFit : 8;
   static constexpr uint32_t kQ0 = 0, kKv0 = 2 * kOp, kRaw0 = kKv0 + kSlots * kOp;
+  static constexpr bool kThinItems = kE4m3 && DC == 2;
   static constexpr size_t kSmem = kRaw0 + (size_t)kRawSlots * kRaw + 1024;
   static_assert(kSlots >= 3, "ring");
 };
@@ -77,14 +83,15 @@ __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two) {
 struct PcItem {
   int row0;        // first row of the tile in its request
   int rows;        // rows of the tile
-  bool wide;
+  bool wide, thin;
   int kt0, T;
   int TA;          // wide: how many of the tiles chain A uses
   int subs_a, subs_b;   // halves of each chain
-  __device__ __forceinline__ PcItem(const PagedArgs& a, const PgItem& it) {
+  __device__ __forceinline__ PcItem(const PagedArgs& a, const PgItem& it, bool thin_items) {
     row0 = it.t * kTile;
     rows = min(kTile, it.r.ql * a.group - row0);
     wide = rows > kRows;
+    thin = thin_items && rows <= kThin;
     kt0 = it.j0;
     T = it.j1 - it.j0;
     const int x0 = (it.r.kl - it.r.ql) * a.group + row0;        // position x group of the first row
@@ -118,6 +125,254 @@ __device__ __forceinline__ int tail_rows(int kl, int kt, int box) {
   return end > 0 && end < kKeys && in ? box - in : 0;
 }
 
+// 8x8 16-bit elements transposed over the warp.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+
+// A thin item, by the eight warps of the softmax groups, each on its own from the ring's tiles as the copies bring
+// them: 16 keys of each tile and all of up to 8 rows, or (over 8 rows) 32 keys and half of the rows.
+//   S^T = K Q^T (16 keys x 8 rows),  O^T += V^T P^T (head_dim x 8 rows), products of 16 x 8 x 16 in registers:
+// K and V are their A operands, straight from the tile (codes turned into float16 on the way: no operand tile is
+// written), Q^T and P^T the B operands, and P^T is S^T's fragment transposed.  What a row needs of a head is one
+// pass over the keys, so nothing but the bytes counts; the tcgen05 products take 128 rows and two hand-overs a
+// tile for the same (a decoding step of 64 sequences of up to 8192 tokens: 226 us with them, 145 like this; 16-bit
+// caches gained nothing, 197 and 201 us: there the bytes count either way).
+template <typename T, class Join>
+__device__ __forceinline__ bool thin_item(const PagedArgs& a, const PgItem& it, const PcItem& g, uint8_t* smem, uint64_t* full,
+                                          uint64_t* empty, uint32_t u, float* ml_s, Join& join) {
+  using L = PcLayout<true, 2>;
+  constexpr bool kOutBf = std::is_same<T, __nv_bfloat16>::value;
+  constexpr float kUp = 7.0f, kGrow = 8.0f;
+  constexpr int NF = L::kRawSlots, D = 128, KS = D / 16;      // KS: 16-element steps of head_dim
+  const int tid = threadIdx.x - 128, w = tid >> 5, lane = tid & 31, gq = lane >> 2, t4 = lane & 3;
+  const bool split = g.rows > 8;
+  const int rb = split ? (w >> 2) * 8 : 0;                   // the warp's first row
+  const int kf = split ? (w & 3) * 32 : w * 16, nb = split ? 2 : 1;   // its first key of a tile, blocks of 16
+  // Q^T: this lane has row rb + gq, 16 elements from 16 t4 and from 16 (t4 + 4), four a step (the order of the codes of
+  // K that the lane reads at once), scaled like the chains' rows
+  uint32_t q[KS][2];
+  float sc = a.scale_log2;
+  {
+    const int r = rb + gq, x = g.row0 + r, tok = x / a.group;
+    const bool in = r < g.rows;
+    const T* src = reinterpret_cast<const T*>(a.q) + (int64_t)(it.r.q0 + tok) * a.q_ts + ((int64_t)it.h * a.group + (x - tok * a.group)) * D;
+    float mx = 0.0f;
+    Vec8<T> v[KS / 2];
+#pragma unroll
+    for (int j = 0; j < KS / 2; ++j) {
+      v[j].w[0] = make_uint4(0u, 0u, 0u, 0u);
+      if (in) v[j].load(src + (t4 + 4 * (j >> 1)) * 16 + (j & 1) * 8);
+      float f[8];
+      v[j].unpack(f);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(f[e]));
+    }
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+    const int e2 = min(max((int)(__float_as_uint(mx) >> 23) - 127, -100), 120);
+    const float up = __int_as_float((127 - e2) << 23);
+#pragma unroll
+    for (int j = 0; j < KS / 2; ++j) {
+      float f[8];
+      v[j].unpack(f);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) q[2 * j + (e >> 1)][e & 1] = pack2h<false>(f[2 * e] * up, f[2 * e + 1] * up);
+    }
+    sc *= __ldg(a.k_scale + it.h) * __int_as_float((127 + e2) << 23);
+  }
+  if (sc == 0.0f) sc = 1e-30f;                               // equal weights
+  // rows of this lane's elements of S^T, P^T and O^T: rb + 2 t4 and the next one
+  const float sc0 = __shfl_sync(0xffffffffu, sc, t4 * 8), sc1 = __shfl_sync(0xffffffffu, sc, t4 * 8 + 4);
+  const int off = it.r.kl - it.r.ql;
+  const int pos0 = min(off + (g.row0 + rb + 2 * t4) / a.group, it.r.kl - 1), pos1 = min(off + (g.row0 + rb + 2 * t4 + 1) / a.group, it.r.kl - 1);
+  const int pos_min = off + (g.row0 + rb) / a.group;
+  // The key of this lane's row of S^T, of a block of 16 (and 8 on): in the order 0 4 1 5 2 6 3 7, and the units of V in
+  // the same one, so that the eight lanes of a 16-byte access meet eight units of the swizzled rows.
+  const int kq = (gq >> 1) + (gq & 1) * 4;
+  float o[KS][4];
+#pragma unroll
+  for (int j = 0; j < KS; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[j][e] = 0.0f;
+  float m0 = -FLT_MAX, m1 = -FLT_MAX, l0 = 0.0f, l1 = 0.0f;  // (-FLT_MAX: nothing seen)
+  bool ok = true;
+#pragma unroll 1
+  for (int i = 0; i < g.T; ++i, u += 2) {
+    const int kb = (g.kt0 + i) * kKeys + kf;                 // the warp's first key
+    float x[2][4];                                           // keys kq, kq + 8 of a block, rows 2 t4, 2 t4 + 1
+    {
+      const uint32_t s = u % NF;
+      if (!warp_wait(&full[s], (u / NF) & 1)) {
+        ok = false;
+        break;
+      }
+      const uint8_t* const tile = smem + L::kRaw0 + s * L::kRaw;
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[n][e] = 0.0f;
+        if (n >= nb) continue;
+        const int k0 = kf + n * 16;
+        float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};               // (two sums: half the chain)
+        uint32_t lo[KS], hi[KS];                       // keys kq and kq + 8: the lane's 16-byte units t4 and t4 + 4
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const uint32_t at = (k0 + kq) * 128 + (((t4 + 4 * j) ^ kq) << 4);
+          *reinterpret_cast<uint4*>(lo + 4 * j) = *reinterpret_cast<const uint4*>(tile + at);
+          *reinterpret_cast<uint4*>(hi + 4 * j) = *reinterpret_cast<const uint4*>(tile + at + 8 * 128);
+        }
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          const uint32_t f[4] = {e4m3x2_to_f16x2(lo[ks]), e4m3x2_to_f16x2(hi[ks]), e4m3x2_to_f16x2(lo[ks] >> 16),
+                                 e4m3x2_to_f16x2(hi[ks] >> 16)};
+          if (ks & 1) mma_k16<false>(y, f, q[ks][0], q[ks][1]);
+          else mma_k16<false>(x[n], f, q[ks][0], q[ks][1]);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[n][e] = (x[n][e] + y[e]) * (e & 1 ? sc1 : sc0);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[s]);
+    }
+    if (kb + 16 * nb - 1 > pos_min) {
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (kb + n * 16 + kq + (e >> 1) * 8 > (e & 1 ? pos1 : pos0)) x[n][e] = -INFINITY;
+    }
+    float b0 = fmaxf(x[0][0], x[0][2]), b1 = fmaxf(x[0][1], x[0][3]);
+    if (split) {
+      b0 = fmaxf(b0, fmaxf(x[1][0], x[1][2]));
+      b1 = fmaxf(b1, fmaxf(x[1][1], x[1][3]));
+    }
+    // the maxima only move when a score is above one by more than 2^8
+    if (__any_sync(0xffffffffu, b0 - kUp > m0 + kGrow || b1 - kUp > m1 + kGrow)) {
+#pragma unroll
+      for (int k = 4; k <= 16; k <<= 1) {
+        b0 = fmaxf(b0, __shfl_xor_sync(0xffffffffu, b0, k));
+        b1 = fmaxf(b1, __shfl_xor_sync(0xffffffffu, b1, k));
+      }
+      const float n0 = b0 - kUp > m0 + kGrow ? b0 - kUp : m0, n1 = b1 - kUp > m1 + kGrow ? b1 - kUp : m1;
+      const float f0 = ex2_approx(m0 - n0), f1 = ex2_approx(m1 - n1);
+      m0 = n0;
+      m1 = n1;
+      l0 *= f0;
+      l1 *= f1;
+#pragma unroll
+      for (int j = 0; j < KS; ++j) {
+        o[j][0] *= f0;
+        o[j][1] *= f1;
+        o[j][2] *= f0;
+        o[j][3] *= f1;
+      }
+    }
+    uint32_t p[2][2];
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      if (n >= nb) continue;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float p0 = ex2_approx(x[n][2 * e] - m0), p1 = ex2_approx(x[n][2 * e + 1] - m1);
+        l0 += p0;
+        l1 += p1;
+        p[n][e] = transpose8(pack2h<false>(p0, p1));
+      }
+    }
+    const uint32_t s = (u + 1) % NF;
+    if (!warp_wait(&full[s], ((u + 1) / NF) & 1)) {
+      ok = false;
+      break;
+    }
+    const uint8_t* const tile = smem + L::kRaw0 + s * L::kRaw;
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      if (n >= nb) continue;
+      const int k0 = kf + n * 16;
+      // V^T: unit kq of keys t4, t4 + 4, t4 + 8 and t4 + 12 (P's 2 t4, 2 t4 + 1 and + 8, + 9); two elements a step
+      uint32_t v[4][4];
+      const int end = it.r.kl - (g.kt0 + i) * kKeys;       // rows from here on are past the last token: zeros
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = k0 + t4 + 4 * e;
+        uint4 y = *reinterpret_cast<const uint4*>(tile + r * 128 + (((kq ^ r) & 7) << 4));
+        if (end < kKeys && r >= end) y = make_uint4(0u, 0u, 0u, 0u);
+        v[e][0] = y.x;
+        v[e][1] = y.y;
+        v[e][2] = y.z;
+        v[e][3] = y.w;
+      }
+#pragma unroll
+      for (int j = 0; j < KS; ++j) {
+        const uint32_t lo = __byte_perm(v[0][j >> 1], v[1][j >> 1], j & 1 ? 0x7362 : 0x5140);
+        const uint32_t hi = __byte_perm(v[2][j >> 1], v[3][j >> 1], j & 1 ? 0x7362 : 0x5140);
+        const uint32_t f[4] = {e4m3x2_to_f16x2(lo), e4m3x2_to_f16x2(lo >> 16), e4m3x2_to_f16x2(hi), e4m3x2_to_f16x2(hi >> 16)};
+        mma_k16<false>(o[j], f, p[n][0], p[n][1]);
+      }
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&empty[s]);
+  }
+  // The warps' results are joined through the second Q tile: O^T as [warp][8 rows][D] with the 16-byte units of a
+  // row exchanged by its number.
+#pragma unroll
+  for (int k = 4; k <= 16; k <<= 1) {
+    l0 += __shfl_xor_sync(0xffffffffu, l0, k);
+    l1 += __shfl_xor_sync(0xffffffffu, l1, k);
+  }
+  ok = join() && ok;                                         // whoever used that tile before is through
+  float* const xo = reinterpret_cast<float*>(smem + L::kQ0 + L::kOp);
+  if (gq == 0) {
+    *reinterpret_cast<float4*>(ml_s + (w * 8 + 2 * t4) * 2) = make_float4(m0, l0, m1, l1);
+  }
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    float* const xr = xo + (w * 8 + 2 * t4 + e) * D;
+#pragma unroll
+    for (int j = 0; j < KS; j += 2)
+      *reinterpret_cast<float4*>(xr + (((kq * 4 + (j >> 1)) ^ t4) << 2)) = make_float4(o[j][e], o[j][e + 2], o[j + 1][e], o[j + 1][e + 2]);
+  }
+  ok = join() && ok;
+  const bool whole = it.whole();
+  const float vsc = __ldg(a.v_scale + it.h);
+  const int64_t slot = 2 * (int64_t)blockIdx.x + (it.j0 == 0 ? 1 : 0);
+  for (int x = tid; ok && x < g.rows * (D / 4); x += 256) {
+    const int r = x / (D / 4), d4 = x % (D / 4), w0 = split ? (r >> 3) * 4 : 0, wn = split ? 4 : 8;
+    float mj = -FLT_MAX, lj = 0.0f;
+    for (int k = 0; k < wn; ++k) mj = fmaxf(mj, ml_s[((w0 + k) * 8 + (r & 7)) * 2]);
+    float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+    for (int k = 0; k < wn; ++k) {
+      const float2 ml = *reinterpret_cast<const float2*>(ml_s + ((w0 + k) * 8 + (r & 7)) * 2);
+      const float4 v = *reinterpret_cast<const float4*>(xo + ((w0 + k) * 8 + (r & 7)) * D + ((d4 ^ ((r >> 1) & 3)) << 2));
+      const float f = ex2_approx(ml.x - mj);
+      lj += ml.y * f;
+      y.x += v.x * f;
+      y.y += v.y * f;
+      y.z += v.z * f;
+      y.w += v.w * f;
+    }
+    const float fin = whole ? (lj == 0.0f ? 0.0f : vsc / lj) : vsc;
+    y = make_float4(y.x * fin, y.y * fin, y.z * fin, y.w * fin);
+    if (whole) {
+      const int x0 = g.row0 + r, tok = x0 / a.group;
+      const int64_t orow = (int64_t)(it.r.q0 + tok) * a.hq + (int64_t)it.h * a.group + (x0 - tok * a.group);
+      *reinterpret_cast<uint2*>(reinterpret_cast<T*>(a.out) + orow * D + d4 * 4) = make_uint2(pack2h<kOutBf>(y.x, y.y), pack2h<kOutBf>(y.z, y.w));
+      if (a.lse && d4 == 0) a.lse[orow] = (mj + log2f(lj)) * kPgLn2;
+    } else {
+      *reinterpret_cast<float4*>(a.part_o + (slot * kTile + r) * D + d4 * 4) = y;
+      if (d4 == 0) {
+        a.part_ml[slot * 2 * kTile + r] = mj == -FLT_MAX ? -INFINITY : mj;
+        a.part_ml[slot * 2 * kTile + kTile + r] = lj;
+      }
+    }
+  }
+  return join() && ok;                                       // before the next item's results overwrite these
+}
+
 template <typename T, bool kE4m3, int DC>
 __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __grid_constant__ CUtensorMap tk,
                                                                        const __grid_constant__ CUtensorMap tv,
@@ -132,18 +387,21 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_u32(smem);
   __shared__ uint64_t kv_full[NS], kv_empty[NS], tail_full[kE4m3 ? 1 : NS],
-      raw_full[kE4m3 ? NR : 1], raw_empty[kE4m3 ? NR : 1],
+      raw_full[kE4m3 ? NR : 1], raw_empty[kE4m3 ? NR : 1], thin_empty[kE4m3 ? NR : 1],
       q_full, q_empty, s_full[4], p_full[4], pv_done[4], mma_done[2], joined,   // s, p, pv: [2 * chain + buffer]
       sc_full[kE4m3 ? 2 : 1], q_seen[kE4m3 ? 2 : 1];   // an item's row scales are there, have been read: by item parity
   __shared__ uint32_t tmem_base_s;
   __shared__ volatile int s_abort;
+  __shared__ volatile uint32_t thin_done;        // thin items whose results are joined
   __shared__ PgShare share;
   __shared__ int64_t scan[kThreads / 32];
-  __shared__ float join_s[2][kRows];             // [chain][row]: maxima, then sums, at the end of a deep item
+  __shared__ __align__(16) float join_s[2][kRows];             // [chain][row]: maxima, then sums, at the end of a deep item
   __shared__ int8_t qexp_s[2][kE4m3 ? kTile : 1];   // e of a row's Q scale 2^-e, by item parity
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const PgTiles tiles{kTile, kKeys, a.group};
+  // codes: rows of 128, so that the raw tiles have the 128-byte swizzle (make_page_map)
+  const bool thin_items = L::kThinItems && a.D == 128;
   if (threadIdx.x == 0) {
     for (int s = 0; s < NS; ++s) {
       mbar_init(&kv_full[s], kE4m3 ? 4 : 1);
@@ -154,6 +412,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
       mbar_init(&raw_full[s], 1);
       mbar_init(&raw_empty[s], 4);
     }
+    for (int s = 0; s < NR; ++s) mbar_init(&thin_empty[s], 8);
     mbar_init(&q_full, 4);
     mbar_init(&q_empty, 2);
     for (int c = 0; c < 4; ++c) {
@@ -169,6 +428,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
       mbar_init(&q_seen[x], 8);
     }
     s_abort = 0;
+    thin_done = 0;
     fence_mbar_init();
     asm volatile("prefetch.tensormap [%0];" ::"l"(&tk) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&tv) : "memory");
@@ -193,7 +453,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
   PgWalk walk(share);
   PgItem it;
 
-  if (warp == 0) {
+  if (warp == 0 || (kE4m3 && warp == 3)) {
     // ---------------------------------------------------------------- TMA producer
     // A tile is kKeys / box boxes of `box` keys, each inside one page; lane l serves box l % boxes.
     const int boxes = kKeys / box;
@@ -204,9 +464,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
     constexpr uint32_t kSlotBytes = kE4m3 ? L::kRaw : L::kOp;
     const uint32_t bytes = kE4m3 ? (uint32_t)(kKeys * D) : kSlotBytes;
     uint32_t u = 0;                                            // copies so far = tiles of the ring used
+    uint32_t by_thin = 0, e_par = 0, t_par = 0;                // codes, by slot: whose release to wait for, and its parity
     bool ok = true;
     while (ok && walk.next(a, tiles, it)) {
-      const PcItem g(a, it);
+      const PcItem g(a, it, thin_items);
       const int32_t* bt = a.block_table + (int64_t)it.b * a.bt_stride;
       auto page_of = [&](int kt, int& in) -> int {             // block and row of this lane's box of tile kt
         const int key = kt * kKeys + bx * box;
@@ -227,8 +488,19 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
         if (i + 1 < g.T) phys_next = page_of(g.kt0 + i + 1, in_next);
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv, ++u) {
+          if (kE4m3 && kv != (warp == 3)) continue;            // codes: K by warp 0, V by warp 3
           const uint32_t s = u % NF;
-          if (u >= NF && !warp_wait(&empty[s], ((u / NF) & 1) ^ 1)) s_abort = 1;
+          if constexpr (L::kThinItems) {
+            const uint32_t bit = 1u << s;
+            const bool by = by_thin & bit;
+            if (u >= NF) {
+              if (!warp_wait(by ? &thin_empty[s] : &empty[s], ((by ? t_par : e_par) >> s) & 1)) s_abort = 1;
+              (by ? t_par : e_par) ^= bit;
+            }
+            by_thin = g.thin ? by_thin | bit : by_thin & ~bit;
+          } else {
+            if (u >= NF && !warp_wait(&empty[s], ((u / NF) & 1) ^ 1)) s_abort = 1;
+          }
           if (__any_sync(0xffffffffu, s_abort)) {
             ok = false;
             break;
@@ -264,7 +536,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
       }
     }
     // every copy this CTA issued has landed before it exits (tails: warp 3 has seen theirs)
-    for (uint32_t v = u > NF ? u - NF : 0; v < u; ++v) mbar_wait_bounded(&full[v % NF], (v / NF) & 1);
+    for (uint32_t v = u > NF ? u - NF : 0; v < u; ++v)
+      if (!kE4m3 || (v & 1) == (warp == 3)) mbar_wait_bounded(&full[v % NF], (v / NF) & 1);
   } else if (warp <= 2) {
     // ---------------------------------------------------------------- MMA issuers: warp 1 + c, chain c
     {
@@ -276,7 +549,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
       uint32_t n = 0;                                          // halves of the chain whose S has been issued, all items
       bool ok = true;
       while (ok && walk.next(a, tiles, it)) {
-        const PcItem g(a, it);
+        const PcItem g(a, it, thin_items);
+        if (g.thin) continue;                                  // (the warps of the softmax groups do it all)
         const int subs = g.subs(c);
         const uint64_t qd = desc_kmajor(sbase + L::kQ0 + (g.wide ? c : 0) * L::kOp);
         auto issue_s = [&](int m) -> bool {
@@ -345,7 +619,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
       uint32_t u = 0, seen = 0;                                // parity of each slot's tail barrier
       bool ok = true;
       while (ok && walk.next(a, tiles, it)) {
-        const PcItem g(a, it);
+        const PcItem g(a, it, thin_items);
         const int i = it.r.kl / kKeys - g.kt0;                 // the tile with the first row past the last token
         const int rows = i >= 0 && i < g.T ? tail_rows(it.r.kl, g.kt0 + i, box) : 0;
         if (rows > 0) {
@@ -369,10 +643,24 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
   } else if (warp >= 12) {
     // ---------------------------------------------------------------- helpers: query rows, e4m3 codes to float16
     const int ht = threadIdx.x - 384;                                     // 0 .. 127
-    uint32_t u = 0, item = 0;
+    uint32_t u = 0, ur = 0, item = 0, thin = 0;                           // positions in the operand ring and in the raw one
     bool ok = true;
     while (ok && walk.next(a, tiles, it)) {
-      const PcItem g(a, it);
+      const PcItem g(a, it, thin_items);
+      if (g.thin) {
+        ur += 2 * g.T;
+        ++thin;
+        continue;
+      }
+      // the second Q tile is where the thin items before this one join their results
+      if (g.wide) {
+        const uint64_t t0 = globaltimer_ns();
+        while (__any_sync(0xffffffffu, thin_done != thin) && !__any_sync(0xffffffffu, s_abort))
+          if (__any_sync(0xffffffffu, globaltimer_ns() - t0 > g_wait_limit_ns)) {
+            atomicOr(&g_tu_status, kStatusWaitTimeout);
+            s_abort = 1;
+          }
+      }
       if (item > 0 && !warp_wait(&q_empty, (item - 1) & 1)) s_abort = 1;
       // S of a short item, and so q_empty, may be done while the softmax still is an item or two back: its row scales
       // stay until it has read them (and have barriers of their own by item parity: a warp that is late cannot tell
@@ -446,9 +734,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
       if constexpr (kE4m3) {
         const uint32_t pitch = ((uint32_t)(box * D) + 127u) & ~127u;
         const int lbox = __ffs(box) - 1;
-        for (int i = 0; i < 2 * g.T && ok; ++i, ++u) {
-          const uint32_t sr = u % NR, s = u % NS;
-          if (!warp_wait(&raw_full[sr], (u / NR) & 1)) s_abort = 1;
+        for (int i = 0; i < 2 * g.T && ok; ++i, ++u, ++ur) {
+          const uint32_t sr = ur % NR, s = u % NS;
+          if (!warp_wait(&raw_full[sr], (ur / NR) & 1)) s_abort = 1;
           if (u >= NS && !warp_wait(&kv_empty[s], ((u / NS) & 1) ^ 1)) s_abort = 1;
           if (__any_sync(0xffffffffu, s_abort)) {
             ok = false;
@@ -462,13 +750,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
           // stores cover a row's eight units, and the swizzle (r & 7) is the thread's own.
           constexpr int UPR = 8 * DC, step = kHelpers / UPR;      // units a row, rows a pass (a multiple of 8)
           const int q = ht % UPR, r0 = ht / UPR;
+          const int qb = D == 128 ? ((((q >> 1) ^ r0) & 7) << 4) + (q & 1) * 8 : q * 8;   // of the unit in its row of codes
           uint8_t* const d0 = dst + (q >> 3) * kChunkBytes + r0 * 128 + (((q & 7) ^ (r0 & 7)) << 4);
           auto put = [&](uint8_t* d, uint2 x) {
             *reinterpret_cast<uint4*>(d) =
                 make_uint4(e4m3x2_to_f16x2(x.x), e4m3x2_to_f16x2(x.x >> 16), e4m3x2_to_f16x2(x.y), e4m3x2_to_f16x2(x.y >> 16));
           };
           if (D == 64 * DC && end >= kKeys) {                     // whole tiles of whole chunks: rows one after another
-            const uint8_t* const r8 = raw + r0 * (64 * DC) + q * 8;
+            const uint8_t* const r8 = raw + r0 * (64 * DC) + qb;
 #pragma unroll
             for (int k = 0; k < kKeys / step; k += 8) {
               uint2 x[8];
@@ -480,7 +769,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
           } else if (q * 8 < D) {
             for (int r = r0; r < kKeys; r += step) {
               uint2 x = make_uint2(0u, 0u);
-              if (r < end) x = *reinterpret_cast<const uint2*>(raw + (r >> lbox) * pitch + (r & (box - 1)) * D + q * 8);
+              if (r < end) x = *reinterpret_cast<const uint2*>(raw + (r >> lbox) * pitch + (r & (box - 1)) * D + qb);
               put(d0 + (r - r0) * 128, x);
             }
           }
@@ -502,7 +791,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
     const uint32_t s_col = tmem + lane_addr + (uint32_t)c * 256u, o_col = s_col + 128u;
     uint32_t n = 0, item = 0;                              // halves of the chain so far; items
     int64_t at = walk.at;                                  // first unit of the item's part
-    uint32_t joins = 0;
+    uint32_t joins = 0, u = 0;                             // u: position in the ring of the copies
     bool ok = true;
     auto join = [&]() -> bool {                            // a barrier of the two groups, bounded like every wait
       tc_fence_before();
@@ -514,7 +803,23 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
       return met;
     };
     while (ok && walk.next(a, tiles, it)) {
-      const PcItem g(a, it);
+      const PcItem g(a, it, thin_items);
+      if constexpr (L::kThinItems) {
+        if (g.thin) {
+          if (!thin_item<T>(a, it, g, smem, raw_full, thin_empty, u, &join_s[0][0], join)) {
+            s_abort = 1;
+            ok = false;
+          }
+          if (threadIdx.x == 128) {                          // (behind the last join)
+            thin_done = thin_done + 1;
+            if (!it.whole() && it.j0 == 0) a.cut[blockIdx.x] = make_int4(g.row0, it.b, it.h, pg_cta_of(at + it.n - 1, share.total, share.ctas));
+          }
+          u += 2 * g.T;
+          at += it.j1 - it.j0;
+          continue;
+        }
+      }
+      u += 2 * g.T;
       const int trow = (g.wide ? c * kRows : 0) + row;     // row of the tile
       const bool valid = trow < g.rows;
       const bool any_valid = (g.wide ? c * kRows : 0) + quarter * 32 < g.rows;
@@ -718,7 +1023,7 @@ int make_page_map(CUtensorMap* map, const void* base, bool e4m3, bool bf16, cons
   cuuint32_t estr[4] = {1, 1, 1, 1};
   CUresult r = fn(map, e4m3 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
                   4, const_cast<void*>(base), dims, strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  e4m3 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  e4m3 && a.D != 128 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, e4m3 ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B : CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return set_error(KVB_E_LAUNCH, "paged_prefill_attention: tensor map failed (%d)", (int)r);
   return KVB_OK;

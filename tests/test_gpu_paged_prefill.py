@@ -235,6 +235,15 @@ def test_many_requests():
     Case(15, chunks.tolist(), contexts.tolist(), 2, 1, 32, 16, "fp32").check(0)
 
 
+@pytest.mark.parametrize("dt", ["bf16", "fp16"])
+@pytest.mark.parametrize("bs,scale", [(16, None), (4, -0.1), (128, 0.0)])
+def test_few_rows_between_long_chunks_over_codes(dt, bs, scale):
+    """Items of up to 16 rows go past the tensor-memory chains and share their buffers with what runs before and after."""
+    chunks = [1, 300, 2, 1, 40, 65, 3, 300, 4, 1, 0, 1, 5, 257, 2]
+    contexts = [1000, 700, 2, 129, 41, 1300, 128, 301, 2000, 127, 60, 0, 3, 900, 4097]
+    Case(13, chunks, contexts, 8, 2, 128, bs, dt, "e4m3").check(2, scale=scale)
+
+
 @pytest.mark.parametrize("tokens", [1, 2, 40])
 def test_many_short_requests_over_codes_keep_their_row_scales(tokens):
     """Short items follow one another in a CTA faster than their softmax; each row has a scale of its own."""
