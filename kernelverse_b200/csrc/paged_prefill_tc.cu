@@ -655,8 +655,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
         ++thin;
         continue;
       }
-      // the second Q tile is where the thin items before this one join their results
-      if (g.wide) {
+      // The thin items before this one are through: they join their results in the second Q tile, and the raw ring's
+      // barriers went on without this warp (a wait cannot tell a phase from the second next).
+      if constexpr (L::kThinItems) {
         const uint64_t t0 = globaltimer_ns();
         while (__any_sync(0xffffffffu, thin_done != thin) && !__any_sync(0xffffffffu, s_abort))
           if (__any_sync(0xffffffffu, globaltimer_ns() - t0 > g_wait_limit_ns)) {
@@ -809,6 +810,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
       const PcItem g(a, it, thin_items);
       if constexpr (L::kThinItems) {
         if (g.thin) {
+          // (this warp's last wait of the item before followed all its raw tiles but one of K and V at most, and the ring
+          // has room for two: the phases that it has not seen are over)
           if (!thin_item<T>(a, it, g, smem, raw_full, thin_empty, u, &join_s[0][0], join)) {
             s_abort = 1;
             ok = false;

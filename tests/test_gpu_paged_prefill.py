@@ -244,6 +244,16 @@ def test_few_rows_between_long_chunks_over_codes(dt, bs, scale):
     Case(13, chunks, contexts, 8, 2, 128, bs, dt, "e4m3").check(2, scale=scale)
 
 
+@pytest.mark.parametrize("seed,group", [(14, 4), (15, 1), (16, 8)])
+def test_few_and_many_rows_in_turn_over_codes(seed, group):
+    """Several items of every kind in each CTA, in random order: whoever skips an item meets the next one's buffers
+    only when they are that one's."""
+    rng = seeded(seed)
+    chunks = [int(c) for c in rng.choice([1, 1, 2, 5, 20, 40, 130, 300], 240)]
+    contexts = [c + int(rng.integers(0, 900)) for c in chunks]
+    Case(seed, chunks, contexts, 2 * group, 2, 128, 16, "bf16", "e4m3").check(2)
+
+
 @pytest.mark.parametrize("tokens", [1, 2, 40])
 def test_many_short_requests_over_codes_keep_their_row_scales(tokens):
     """Short items follow one another in a CTA faster than their softmax; each row has a scale of its own."""
