@@ -475,6 +475,21 @@ KVB_API int kvb_paged_prefill_attention_variant(const void* q, int q_dtype, int6
                                                 void* stream);
 
 /*
+ * Test hooks of the division of kvb_paged_prefill_attention's work, on the host (no GPU call; no
+ * reference counterpart), for a request of q_len new tokens and seq_len tokens whose KV heads have
+ * `group` query heads.
+ * _units: out[3] = tiles of `rows` query rows (of one KV head), units of `keys` keys of tile `tile`,
+ * units of the tiles before it (`tile` may be the number of tiles: the request's total).
+ * _item: how the tcgen05 kernel works off units [unit0, unit1) of a tile; few_rows: codes of head_dim
+ * 128.  out[7] = kind (0 few rows, 1 deep, 2 wide), rows, key tiles, key tiles that chain A and chain B go
+ * through, halves of them that each goes through.
+ * _cta_of: the CTA that unit `unit` of `units` falls to, of `ctas`; -1 for arguments out of range.
+ */
+KVB_API int kvb_selftest_paged_units(int q_len, int seq_len, int group, int rows, int keys, int tile, int64_t* out);
+KVB_API int kvb_selftest_paged_item(int q_len, int seq_len, int group, int few_rows, int tile, int unit0, int unit1, int* out);
+KVB_API int kvb_selftest_paged_cta_of(int64_t unit, int64_t units, int ctas);
+
+/*
  * Allocation-free variant of kvb_paged_attention (no counterpart in the reference).
  * Some callers cannot allocate device memory: a plugin that its host framework hands only
  * input and output buffers, or a serving loop that must not call cudaMalloc (which can

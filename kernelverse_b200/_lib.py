@@ -60,6 +60,9 @@ SIGNATURES = {
     "kvb_paged_prefill_attention_variant": (_I, [_P, _I, _I64, _P, _P, _I, _I64, _I64, _P, _P, _P, _P, _I, _P, _I64,
                                                 _I, _I64, _I, _I, _I, _I, _I64, _I64, _F, _P, _P, _I, _P, _SZ, _P]),
     "kvb_paged_prefill_attention_workspace_size": (_SZ, [_I]),
+    "kvb_selftest_paged_units": (_I, [_I, _I, _I, _I, _I, _I, _P]),
+    "kvb_selftest_paged_item": (_I, [_I, _I, _I, _I, _I, _I, _I, _P]),
+    "kvb_selftest_paged_cta_of": (_I, [_I64, _I64, _I]),
     "kvb_paged_attention_noalloc": (_I, [_P, _I, _P, _P, _I, _P, _P, _P, _I, _P, _I64, _I, _I, _I, _I, _I, _I64, _I64,
                                          _F, _P, _P, _I, _I, _P, _I, _P, _P, _P, _I, _P]),
 }

@@ -61,7 +61,7 @@ __device__ __forceinline__ bool pg_request(const PagedArgs& a, int b, PgRequest&
 
 // sum over t in [0, n) of floor((b + s t) / m), b >= 0, s, m > 0, all numerators below 2^31
 // (the Euclid-like recursion on (s, m)).
-__device__ __forceinline__ int64_t pg_floor_sum(uint32_t n, uint32_t m, uint32_t s, uint32_t b) {
+__host__ __device__ __forceinline__ int64_t pg_floor_sum(uint32_t n, uint32_t m, uint32_t s, uint32_t b) {
   int64_t ans = 0;
   while (n > 0) {
     ans += (int64_t)(n - 1) * n / 2 * (s / m) + (int64_t)n * (b / m);
@@ -83,15 +83,15 @@ __device__ __forceinline__ int64_t pg_floor_sum(uint32_t n, uint32_t m, uint32_t
 // so that rows that see nothing are written too.
 struct PgTiles {
   int rt, bku, group;
-  __device__ __forceinline__ int count(const PgRequest& r) const { return (int)(((int64_t)r.ql * group + rt - 1) / rt); }
-  __device__ __forceinline__ int units(const PgRequest& r, int t) const {
+  __host__ __device__ __forceinline__ int count(const PgRequest& r) const { return (int)(((int64_t)r.ql * group + rt - 1) / rt); }
+  __host__ __device__ __forceinline__ int units(const PgRequest& r, int t) const {
     const int rw = r.ql * group;
     const int last = min((t + 1) * rt, rw) - 1;
     const int x = (r.kl - r.ql) * group + last;
     return x < 0 ? 1 : x / (group * bku) + 1;
   }
   // units of tiles [0, t), t <= count
-  __device__ __forceinline__ int64_t before(const PgRequest& r, int t) const {
+  __host__ __device__ __forceinline__ int64_t before(const PgRequest& r, int t) const {
     if (t == 0) return 0;
     const int n = count(r);
     int64_t sum = 0;
@@ -206,7 +206,7 @@ __device__ __forceinline__ void pg_share(const PagedArgs& a, const PgTiles& tile
 struct PgItem {
   PgRequest r;
   int b, h, t, j0, j1, n;
-  __device__ __forceinline__ bool whole() const { return j0 == 0 && j1 == n; }
+  __host__ __device__ __forceinline__ bool whole() const { return j0 == 0 && j1 == n; }
 };
 // Walks the items of a share; every role of a CTA walks the same ones on its own.
 struct PgWalk {
@@ -243,7 +243,7 @@ struct PgWalk {
   }
 };
 // CTA that holds unit x.
-__device__ __forceinline__ int pg_cta_of(int64_t x, int64_t total, int ctas) {
+__host__ __device__ __forceinline__ int pg_cta_of(int64_t x, int64_t total, int ctas) {
   int c = (int)(((x + 1) * ctas - 1) / total);     // floor(total * c / ctas) <= x for this c or the one before
   while (c + 1 < ctas && total * (c + 1) / ctas <= x) ++c;
   while (c > 0 && total * c / ctas > x) --c;

@@ -90,7 +90,7 @@ struct PcItem {
   int kt0, T;
   int TA;          // wide: how many of the tiles chain A uses
   int subs_a, subs_b;   // halves of each chain
-  __device__ __forceinline__ PcItem(const PagedArgs& a, const PgItem& it, bool thin_items) {
+  __host__ __device__ __forceinline__ PcItem(const PagedArgs& a, const PgItem& it, bool thin_items) {
     row0 = it.t * kTile;
     rows = min(kTile, it.r.ql * a.group - row0);
     wide = rows > kRows;
@@ -113,7 +113,9 @@ struct PcItem {
       subs_b = T - (low ? 1 : 0);
     }
   }
-  __device__ __forceinline__ int subs(int c) const { return c ? subs_b : subs_a; }
+  __host__ __device__ __forceinline__ int subs(int c) const { return c ? subs_b : subs_a; }
+  // tiles that the chain goes through: all, or all but the last
+  __host__ __device__ __forceinline__ int tiles(int c) const { return wide ? (c ? T : TA) : subs(c); }
   // tile (of the item) and half of the chain's m-th half
   __device__ __forceinline__ int tile(int m) const { return wide ? m >> 1 : m; }
   __device__ __forceinline__ int half(int c, int m) const { return wide ? m & 1 : c; }
@@ -796,7 +798,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
     uint32_t n = 0, item = 0;                              // halves of the chain so far; items
     int64_t at = walk.at;                                  // first unit of the item's part
     uint32_t joins = 0, u = 0;                             // u: position in the ring of the copies
-    bool ok = true;
+    bool ok = true, after_wide = false;                    // after_wide: the item before was a wide one
     auto join = [&]() -> bool {                            // a barrier of the two groups, bounded like every wait
       tc_fence_before();
       __syncwarp();
@@ -810,8 +812,15 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
       const PcItem g(a, it, thin_items);
       if constexpr (L::kThinItems) {
         if (g.thin) {
-          // (this warp's last wait of the item before followed all its raw tiles but one of K and V at most, and the ring
-          // has room for two: the phases that it has not seen are over)
+          // A parity wait cannot tell a phase from the one two before it, so every raw tile of the items before has to
+          // have landed for certain.  The chain that goes through an item's last tile knows that of all its tiles; a deep
+          // item's groups part from it together, but chain A may leave a wide one without that tile: they meet here.
+          if (after_wide) ok = join();
+          after_wide = false;
+          if (!ok) {
+            s_abort = 1;
+            break;
+          }
           if (!thin_item<T>(a, it, g, smem, raw_full, thin_empty, u, &join_s[0][0], join)) {
             s_abort = 1;
             ok = false;
@@ -826,6 +835,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
         }
       }
       u += 2 * g.T;
+      after_wide = g.wide;
       const int trow = (g.wide ? c * kRows : 0) + row;     // row of the tile
       const bool valid = trow < g.rows;
       const bool any_valid = (g.wide ? c * kRows : 0) + quarter * 32 < g.rows;
@@ -1084,3 +1094,39 @@ int paged_prefill_tcgen05(PagedArgs& a, int q_dtype, int cache_dtype, void* ws, 
 }
 
 }  // namespace kvb
+
+using namespace kvb;
+
+extern "C" int kvb_selftest_paged_item(int q_len, int seq_len, int group, int few_rows, int tile, int unit0, int unit1, int* out) {
+  if (!out || q_len <= 0 || seq_len < 0 || group <= 0 || tile < 0 || unit0 < 0 || unit1 <= unit0)
+    return set_error(KVB_E_ARG, "selftest_paged_item: bad arguments");
+  PagedArgs a{};
+  a.group = group;
+  const PgTiles tiles{kTile, kKeys, group};
+  PgItem it{};
+  it.r = PgRequest{0, q_len, seq_len};
+  it.t = tile;
+  it.j0 = unit0;
+  it.j1 = unit1;
+  if (tile >= tiles.count(it.r) || unit1 > tiles.units(it.r, tile))
+    return set_error(KVB_E_ARG, "selftest_paged_item: no such item");
+  const PcItem g(a, it, few_rows != 0);
+  const int v[7] = {g.thin ? 0 : g.wide ? 2 : 1, g.rows, g.T, g.tiles(0), g.tiles(1), g.subs(0), g.subs(1)};
+  for (int i = 0; i < 7; ++i) out[i] = v[i];
+  return KVB_OK;
+}
+
+extern "C" int kvb_selftest_paged_units(int q_len, int seq_len, int group, int rows, int keys, int tile, int64_t* out) {
+  const PgRequest r{0, q_len, seq_len};
+  const PgTiles tiles{rows, keys, group};
+  if (!out || q_len <= 0 || seq_len < 0 || group <= 0 || rows <= 0 || keys <= 0 || tile < 0 || tile > tiles.count(r))
+    return set_error(KVB_E_ARG, "selftest_paged_units: bad arguments");
+  out[0] = tiles.count(r);
+  out[1] = tile < tiles.count(r) ? tiles.units(r, tile) : 0;
+  out[2] = tiles.before(r, tile);
+  return KVB_OK;
+}
+
+extern "C" int kvb_selftest_paged_cta_of(int64_t unit, int64_t units, int ctas) {
+  return unit < 0 || unit >= units || ctas <= 0 || ctas > units ? -1 : pg_cta_of(unit, units, ctas);
+}

@@ -423,3 +423,16 @@ def test_append_then_attend(dt, cache):
         bound = half * np.abs(ref) + ((2.0 ** -21 if dt == "fp32" else half) + 2 * reach[..., None] * (d * 2.0 ** -23 + 2.0 ** -21)
                                       + 2.0 ** -16) * weight
         assert (np.abs(host(out) - ref) <= bound * 1.01).all()
+
+
+@pytest.mark.parametrize("bs", [16, 128])
+def test_few_rows_right_after_wide_items_over_codes(bs):
+    """Wide items whose last key tile only the lower half of their rows sees, each followed by items of few rows that
+    wrap around the ring of copies: the groups part at different tiles of the one and start the other together."""
+    rng = seeded(40 + bs)
+    chunks, contexts = [], []
+    for _ in range(250):
+        n = int(rng.integers(34, 65))                        # 4 heads: 136 to 256 rows
+        chunks += [n, 1]
+        contexts += [128 * int(rng.integers(1, 6)) + max(1, n - 40), int(rng.integers(129, 900))]
+    Case(41, chunks, contexts, 8, 2, 128, bs, "bf16", "e4m3").check(2)
