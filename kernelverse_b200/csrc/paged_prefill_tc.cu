@@ -121,8 +121,6 @@ struct PcItem {
   __device__ __forceinline__ int half(int c, int m) const { return wide ? m & 1 : c; }
   // whether the chain is done with the tile after its m-th half
   __device__ __forceinline__ bool leaves(int c, int m) const { return !wide || (m & 1) || m + 1 == subs(c); }
-  // whether one chain alone uses tile i
-  __device__ __forceinline__ bool one_user(int i) const { return wide ? i >= TA : i >= subs_b; }
 };
 // Rows of key tile kt past the last token that a box of the tile holds together with tokens.
 __device__ __forceinline__ int tail_rows(int kl, int kt, int box) {
@@ -512,12 +510,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
           }
           const CUtensorMap* map = kv ? &tv : &tk;
           uint64_t* bar = &full[s];
-          if constexpr (!kE4m3) {
-            // a V tile whose last page has rows past the last token goes through warp 3
+          // a V tile whose last page has rows past the last token goes through warp 3
+          if constexpr (!kE4m3)
             if (kv && tail_rows(it.r.kl, g.kt0 + i, box) > 0) bar = &tail_full[s];
-            // the slot's release takes an arrival of each chain: this one stands for a chain that does not use the tile
-            if (lane == 0 && g.one_user(i)) mbar_arrive(&empty[s]);
-          }
           if (lane == 0) mbar_arrive_expect_tx(bar, bytes);
           __syncwarp();
           // box by box in converged code (issued by the lanes of the boxes instead, each took ~105 cycles)
@@ -608,6 +603,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
           }
           __syncwarp();
           if (m + 2 < subs) ok = issue_s(m + 2);
+        }
+        // A tile that only the other chain goes through: seen and passed on all the same.  A wait cannot tell a phase
+        // from the one two before, so this warp sees every phase of every slot, and the slot is not filled again before.
+        for (int v = 2 * g.tiles(c); v < 2 * g.T && ok; ++v) {
+          const uint32_t s = (u0 + v) % NS;
+          ok = warp_wait(&kv_full[s], ((u0 + v) / NS) & 1);
+          if (ok && lane == 0) mbar_arrive(&kv_empty[s]);
         }
         u0 += 2 * g.T;
         if (__any_sync(0xffffffffu, s_abort)) ok = false;
@@ -748,7 +750,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
             ok = false;
             break;
           }
-          if (ht == 0 && g.one_user(i >> 1)) mbar_arrive(&kv_empty[s]);   // for the chain that does not use the tile
           const uint8_t* raw = smem + L::kRaw0 + sr * L::kRaw;
           uint8_t* dst = smem + L::kKv0 + s * L::kOp;
           const int end = it.r.kl - (g.kt0 + (i >> 1)) * kKeys;  // rows from here on are past the last token

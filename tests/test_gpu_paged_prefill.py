@@ -436,3 +436,17 @@ def test_few_rows_right_after_wide_items_over_codes(bs):
         chunks += [n, 1]
         contexts += [128 * int(rng.integers(1, 6)) + max(1, n - 40), int(rng.integers(129, 900))]
     Case(41, chunks, contexts, 8, 2, 128, bs, "bf16", "e4m3").check(2)
+
+
+@pytest.mark.parametrize("dt,d", [("bf16", 128), ("fp16", 64)])
+def test_items_whose_last_tile_one_chain_leaves_out(dt, d):
+    """Wide items whose upper rows, and deep ones whose upper keys, end a tile early, in turn and followed by items that
+    wrap around the ring: each chain's issuer keeps step with the copies."""
+    rng = seeded(42 + d)
+    chunks, contexts = [], []
+    for _ in range(150):
+        n = int(rng.integers(34, 65))
+        chunks += [n, int(rng.integers(1, 30)), 1]
+        contexts += [128 * int(rng.integers(1, 6)) + max(1, n - 40), 128 * int(rng.integers(1, 6)) + int(rng.integers(1, 65)),
+                     int(rng.integers(30, 900))]
+    Case(43, chunks, contexts, 8, 2, d, 16, dt).check(2)

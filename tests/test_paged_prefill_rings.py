@@ -82,3 +82,25 @@ def test_few_row_items_wait_for_no_phase_that_may_lie_two_ahead():
     every = [some_items(seed, 1) for seed in range(400)]
     assert sum(unsound_waits_on_codes(items, False) for items in every) > 0       # what the meeting is for
     assert all(unsound_waits_on_codes(items, True) == 0 for items in every)
+
+
+def unsound_waits_of_issuers(items, see_all, slots):
+    """Waits of the MMA issuers (chain A, chain B) in the ring of 16-bit K and V tiles (K at even positions)."""
+    known, found, u = [set(), set()], 0, 0
+    for it in items:
+        for c, tiles in enumerate((it["A"], it["B"])):
+            for p in range(u, u + 2 * (it["T"] if see_all else tiles)):
+                found += p >= slots and p - slots not in known[c]
+                known[c].add(p)
+        # the next item's query rows come once both chains' products of this one's have read them, and every K
+        for c in range(2):
+            known[c] |= {u + 2 * i for i in range(it["T"])}
+        u += 2 * it["T"]
+    return found
+
+
+@pytest.mark.parametrize("slots", [3, 5, 8])
+def test_issuers_wait_for_no_phase_that_may_lie_two_ahead(slots):
+    every = [some_items(seed, 0) for seed in range(400)]
+    assert sum(unsound_waits_of_issuers(items, False, slots) for items in every) > 0
+    assert all(unsound_waits_of_issuers(items, True, slots) == 0 for items in every)
