@@ -28,7 +28,8 @@
 // What bounds it: for long chunks the chains' hand-overs and the operands of S in shared memory (2048 new
 // tokens of 16384, 32 + 8 heads of 128, bf16: 520-540 us, 0.58 of the bf16 rate; 4 x 512 of 4096 over
 // codes 180-190 us); for decoding over 16-bit caches HBM (64 sequences of 4352 tokens: 197 us, 5.8 TB/s).
-// Every mbarrier wait is bounded; on a timeout the roles stop, the producer waits for its own copies,
+// Every wait is bounded: by a time limit where one hand-over is waited for, by the limit since the last copy was
+// issued where whole items are (a page tail at the end of a share, query rows behind few-row items); on a timeout the roles stop, the producer waits for its own copies,
 // the MMA lanes for their MMAs, and the CTA frees its TMEM before exiting.
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -79,6 +80,41 @@ __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two) {
   const uint16_t v = (uint16_t)two;
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(v));
   return r;
+}
+
+// A wait for the end of whole items, not of one hand-over: it gives up when warp 0 has issued no copy for the limit
+// (whose own waits are for one hand-over each), however long the items in between take.
+struct Patience {
+  volatile uint32_t* copies;     // copies that warp 0 has issued
+  volatile int* abort;
+  uint64_t t0;
+  uint32_t seen;
+  __device__ __forceinline__ Patience(volatile uint32_t* c, volatile int* a) : copies(c), abort(a), t0(globaltimer_ns()), seen(*c) {}
+  __device__ __forceinline__ bool over() {
+    if (*abort) return true;
+    const uint32_t now = *copies;
+    const uint64_t t = globaltimer_ns();
+    if (now != seen) {
+      seen = now;
+      t0 = t;
+    } else if (t - t0 > *(volatile uint64_t*)&g_wait_limit_ns) {
+      atomicOr(&g_tu_status, kStatusWaitTimeout);
+      return true;
+    }
+    return false;
+  }
+};
+// Like warp_wait.
+__device__ __forceinline__ bool patient_wait(uint64_t* bar, uint32_t parity, volatile uint32_t* copies, volatile int* abort) {
+  bool ok = mbar_try_wait(bar, parity);
+  if (!ok) {
+    Patience p(copies, abort);
+    for (uint32_t i = 1; !ok; ++i) {
+      ok = mbar_try_wait(bar, parity);
+      if (!ok && (i & 255u) == 0 && p.over()) break;
+    }
+  }
+  return __all_sync(0xffffffffu, ok);
 }
 
 // What every role derives from an item: key tiles [kt0, kt0 + T) of 128 keys, and the 64-key halves that
@@ -395,6 +431,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
       sc_full[kE4m3 ? 2 : 1], q_seen[kE4m3 ? 2 : 1];   // an item's row scales are there, have been read: by item parity
   __shared__ uint32_t tmem_base_s;
   __shared__ volatile int s_abort;
+  __shared__ volatile uint32_t s_copies;         // copies that warp 0 has issued
   __shared__ volatile uint32_t thin_done;        // thin items whose results are joined
   __shared__ PgShare share;
   __shared__ int64_t scan[kThreads / 32];
@@ -431,6 +468,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
       mbar_init(&q_seen[x], 8);
     }
     s_abort = 0;
+    s_copies = 0;
     thin_done = 0;
     fence_mbar_init();
     asm volatile("prefetch.tensormap [%0];" ::"l"(&tk) : "memory");
@@ -514,6 +552,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
           if constexpr (!kE4m3)
             if (kv && tail_rows(it.r.kl, g.kt0 + i, box) > 0) bar = &tail_full[s];
           if (lane == 0) mbar_arrive_expect_tx(bar, bytes);
+          if (lane == 0 && warp == 0) s_copies = u + 1;
           __syncwarp();
           // box by box in converged code (issued by the lanes of the boxes instead, each took ~105 cycles)
           for (int x = 0; x < boxes; ++x) {
@@ -580,7 +619,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
           ++n;
           return true;
         };
-        ok = warp_wait(&q_full, item & 1);
+        ok = patient_wait(&q_full, item & 1, &s_copies, &s_abort);
         ++item;
         if (subs == 0 && ok && lane == 0) mbar_arrive(&q_empty);
         const uint32_t n0 = n;
@@ -631,7 +670,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
         const int rows = i >= 0 && i < g.T ? tail_rows(it.r.kl, g.kt0 + i, box) : 0;
         if (rows > 0) {
           const uint32_t s = (u + 2 * i + 1) % NS;
-          if (!warp_wait(&tail_full[s], (seen >> s) & 1)) s_abort = 1;
+          if (!patient_wait(&tail_full[s], (seen >> s) & 1, &s_copies, &s_abort)) s_abort = 1;
           seen ^= 1u << s;
           const int end = it.r.kl & (kKeys - 1);
           for (int x = lane; x < rows * 8 * DC; x += 32) {
@@ -662,14 +701,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
       // The thin items before this one are through: they join their results in the second Q tile, and the raw ring's
       // barriers went on without this warp (a wait cannot tell a phase from the second next).
       if constexpr (L::kThinItems) {
-        const uint64_t t0 = globaltimer_ns();
-        while (__any_sync(0xffffffffu, thin_done != thin) && !__any_sync(0xffffffffu, s_abort))
-          if (__any_sync(0xffffffffu, globaltimer_ns() - t0 > g_wait_limit_ns)) {
-            atomicOr(&g_tu_status, kStatusWaitTimeout);
+        Patience p(&s_copies, &s_abort);
+        while (__any_sync(0xffffffffu, thin_done != thin))
+          if (__any_sync(0xffffffffu, p.over())) {
             s_abort = 1;
+            break;
           }
       }
-      if (item > 0 && !warp_wait(&q_empty, (item - 1) & 1)) s_abort = 1;
+      if (item > 0 && !patient_wait(&q_empty, (item - 1) & 1, &s_copies, &s_abort)) s_abort = 1;
       // S of a short item, and so q_empty, may be done while the softmax still is an item or two back: its row scales
       // stay until it has read them (and have barriers of their own by item parity: a warp that is late cannot tell
       // phase k of one barrier from phase k + 2)

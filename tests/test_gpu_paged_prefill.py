@@ -450,3 +450,35 @@ def test_items_whose_last_tile_one_chain_leaves_out(dt, d):
         contexts += [128 * int(rng.integers(1, 6)) + max(1, n - 40), 128 * int(rng.integers(1, 6)) + int(rng.integers(1, 65)),
                      int(rng.integers(30, 900))]
     Case(43, chunks, contexts, 8, 2, d, 16, dt).check(2)
+
+
+@pytest.mark.parametrize("cache", ["bf16", "e4m3"])
+def test_launches_longer_than_the_wait_limit(cache):
+    """The limit of a wait is for one hand-over, not for a CTA's whole share.  A long prompt whose page tail comes last
+    (16-bit caches), and wide items behind many of few rows (codes), with the limit far below the launch's duration."""
+    from kernelverse_b200 import _lib
+    ops, d, hkv, bs = _ops(), 128, 8, 16
+    chunks, contexts = ([49151], [49151]) if cache == "bf16" else ([1] * 600 + [64, 64], [65536] * 600 + [300, 300])
+    g = torch.Generator(device="cuda").manual_seed(1)
+    pages = -(-max(contexts) // bs)
+    kv = torch.randn((pages, 2, bs, hkv, d), generator=g, device="cuda")
+    kv = kv.to(torch.bfloat16 if cache == "bf16" else torch.float8_e4m3fn)
+    one = None if cache == "bf16" else torch.ones(hkv, device="cuda")
+    q = torch.randn((sum(chunks), 32, d), generator=g, device="cuda").to(torch.bfloat16)
+    bt = torch.arange(pages, dtype=torch.int32, device="cuda").expand(len(chunks), pages)       # shared pages
+    qo = dev(np.concatenate([[0], np.cumsum(chunks)]).astype(np.int32))
+    lens = dev(np.array(contexts, np.int32))
+    run = lambda: ops.paged_prefill_attention(q, kv[:, 0], kv[:, 1], qo, lens, bt, k_scale=one, v_scale=one, _variant=2)  # noqa: E731
+    want = run()
+    begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    assert _lib.lib().kvb_device_status(1) == 0
+    try:
+        _lib.call("kvb_set_wait_limit_ns", 2_000_000)
+        begin.record()
+        got = run()
+        end.record()
+        assert _lib.lib().kvb_device_status(1) == 0
+    finally:
+        _lib.call("kvb_set_wait_limit_ns", 0)
+    assert begin.elapsed_time(end) > 6.0                     # ms: what the test is about
+    assert torch.equal(got, want)
