@@ -707,6 +707,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
             s_abort = 1;
             break;
           }
+        __threadfence_block();
       }
       if (item > 0 && !patient_wait(&q_empty, (item - 1) & 1, &s_copies, &s_abort)) s_abort = 1;
       // S of a short item, and so q_empty, may be done while the softmax still is an item or two back: its row scales
@@ -866,6 +867,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(const __g
             ok = false;
           }
           if (threadIdx.x == 128) {                          // (behind the last join)
+            __threadfence_block();                           // what the joins ordered before this, for who reads the count
             thin_done = thin_done + 1;
             if (!it.whole() && it.j0 == 0) a.cut[blockIdx.x] = make_int4(g.row0, it.b, it.h, pg_cta_of(at + it.n - 1, share.total, share.ctas));
           }
