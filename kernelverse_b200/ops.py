@@ -667,10 +667,12 @@ def paged_prefill_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     if q1 != 1 or qh != d or (qt * q.element_size()) % 16 or q.data_ptr() % 16:
         q = q.contiguous()
         qt = q.stride(0)
+    width = block_table.shape[1]
+    if max_seq_len is None:
+        max_seq_len = width * bs
     t0, t1 = block_table.stride()
-    if t1 != 1 or t0 < block_table.shape[1]:
-        block_table = block_table.contiguous()
-        t0 = block_table.shape[1]
+    if t1 != 1 or t0 < width or max_seq_len > width * bs:   # (the entry holds max_seq_len against the row stride)
+        block_table, t0 = block_table.contiguous(), width
     qo_indptr, seq_lens = qo_indptr.contiguous(), seq_lens.contiguous()
     lse = q.new_empty((tq, hq), dtype=torch.float32) if return_lse else None
     # per call, from the caching allocator: calls on other streams and captured graphs do not share it
@@ -678,8 +680,7 @@ def paged_prefill_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     ws = q.new_empty((ws_bytes,), dtype=torch.uint8)
     call("kvb_paged_prefill_attention_variant", q.data_ptr(), _DT[q.dtype], qt, k_cache.data_ptr(), v_cache.data_ptr(), cdt,
          ks, vs, _ptr(k_scale), _ptr(v_scale), qo_indptr.data_ptr(), seq_lens.data_ptr(), _INDEX[seq_lens.dtype],
-         block_table.data_ptr(), t0, b, tq, hq, hkv, d, bs, nb,
-         block_table.shape[1] * bs if max_seq_len is None else max_seq_len, d ** -0.5 if scale is None else scale,
+         block_table.data_ptr(), t0, b, tq, hq, hkv, d, bs, nb, max_seq_len, d ** -0.5 if scale is None else scale,
          out.data_ptr(), _ptr(lse), _variant, ws.data_ptr(), ws_bytes, _raw_stream(dev))
     return (out, lse) if return_lse else out
 
