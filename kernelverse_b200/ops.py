@@ -665,8 +665,8 @@ def paged_prefill_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     k_scale, v_scale = _cache_scales(what, cdt, hkv, k_scale, v_scale)
     qt, qh, q1 = q.stride()
     if q1 != 1 or qh != d or (qt * q.element_size()) % 16 or q.data_ptr() % 16:
-        q = q.contiguous()
-        qt = q.stride(0)
+        q = q.clone(memory_format=torch.contiguous_format)     # (contiguous() keeps the strides of a single token's row)
+        qt = hq * d
     width = block_table.shape[1]
     if max_seq_len is None:
         max_seq_len = width * bs

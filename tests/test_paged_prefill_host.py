@@ -62,3 +62,15 @@ def test_lengths_past_other_views_are_refused(attend):
         assert attend(block_table=table, max_seq_len=48)[MAX_LEN] == 48
         with pytest.raises(RuntimeError, match="max_seq_len"):
             attend(block_table=table, max_seq_len=49)
+
+
+@pytest.mark.parametrize("tokens", [1, 3])
+def test_queries_off_the_16_byte_grid_are_copied(attend, tokens):
+    """Rows of an odd width, one token's too (whose stride torch takes for contiguous), and a base between boundaries."""
+    qo = torch.tensor([0, tokens, tokens], dtype=torch.int32)
+    odd = torch.zeros(tokens * 259, dtype=torch.bfloat16).as_strided((tokens, 4, 64), (259, 64, 1))
+    base = torch.zeros(tokens * 256 + 8, dtype=torch.bfloat16)
+    at = next(i for i in range(8) if (base.data_ptr() + 2 * i) % 16 == 2)
+    for q in (odd, base[at:at + tokens * 256].view(tokens, 4, 64)):
+        args = attend(q=q, qo_indptr=qo)
+        assert args[2] == 256 and args[Q] % 16 == 0 and args[Q] != q.data_ptr()
