@@ -208,10 +208,7 @@ __global__ void __launch_bounds__(kRopeThreads, HPT == 1 ? 1 : kRopeBlocks) qk_r
   constexpr int P = V / 2;
   uint64_t c[P], s[P];
 #pragma unroll
-  for (int i = 0; i < P; ++i) {
-    c[i] = f2_pack(1.0f, 1.0f);
-    s[i] = 0ull;
-  }
+  for (int i = 0; i < P; ++i) c[i] = s[i] = 0ull;
   if (pos_ok && active && h0 < a.hq + a.hkv) {
     const float* row = a.cos_sin + pos * a.R;
     if (!a.interleaved) {
@@ -273,13 +270,16 @@ __global__ void __launch_bounds__(kRopeThreads, HPT == 1 ? 1 : kRopeBlocks) qk_r
           for (int e = 0; e < P; ++e) fb[e] = f2_mul(f2_mul(fb[e], r2), wf[e]);
         }
       }
+      // Only vectors that rotate: an element past the rotary dim passes, whatever its lane's other elements are.
       if (!a.interleaved) {
-        const uint64_t minus = f2_pack(-1.0f, -1.0f);
+        if (rot_a) {
+          const uint64_t minus = f2_pack(-1.0f, -1.0f);
 #pragma unroll
-        for (int e = 0; e < P; ++e) {
-          const uint64_t y = fa[e], z = fb[e];
-          fa[e] = f2_fma(y, c[e], f2_mul(f2_mul(z, s[e]), minus));
-          fb[e] = f2_fma(z, c[e], f2_mul(y, s[e]));
+          for (int e = 0; e < P; ++e) {
+            const uint64_t y = fa[e], z = fb[e];
+            fa[e] = f2_fma(y, c[e], f2_mul(f2_mul(z, s[e]), minus));
+            fb[e] = f2_fma(z, c[e], f2_mul(y, s[e]));
+          }
         }
       } else {
         // (y, z) -> (y, z) c + (-z, y) s; pair e of the lane has component e of c and s
@@ -288,10 +288,13 @@ __global__ void __launch_bounds__(kRopeThreads, HPT == 1 ? 1 : kRopeBlocks) qk_r
           const float ce = e & 1 ? c2.y : c2.x, se = e & 1 ? s2.y : s2.x;
           return f2_fma(yz, f2_pack(ce, ce), f2_mul(f2_pack(-v.y, v.x), f2_pack(se, se)));
         };
+        if (rot_a) {
 #pragma unroll
-        for (int e = 0; e < P; ++e) {
-          fa[e] = turn(fa[e], e);
-          fb[e] = turn(fb[e], P + e);
+          for (int e = 0; e < P; ++e) fa[e] = turn(fa[e], e);
+        }
+        if (rot_b) {
+#pragma unroll
+          for (int e = 0; e < P; ++e) fb[e] = turn(fb[e], P + e);
         }
       }
       if (!pos_ok) {

@@ -294,3 +294,58 @@ def test_captured_and_replayed_on_another_stream():
         want = ops.rope_paged_kv_append(q, k, v, kc2, vc2, slots, pos, table, ks, ks)
     s.synchronize()
     assert torch.equal(qo, want) and torch.equal(kc, kc2) and torch.equal(vc, vc2)
+
+
+def _special(x):
+    """Infinities, NaN and signed zeros strewn over the elements."""
+    n = torch.arange(x.numel(), device=x.device).view(x.shape)
+    for k, value in enumerate((float("inf"), float("-inf"), float("nan"), -0.0, 0.0)):
+        x = torch.where(n % 11 == 2 * k, torch.full_like(x, value), x)
+    return x
+
+
+def _same(a, b):
+    """Equal values and signs of zeros; NaN equals NaN."""
+    a, b = a.float(), b.float()
+    return bool((((a == b) & (a.signbit() == b.signbit())) | (a.isnan() & b.isnan())).all())
+
+
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("t", [5, 3000])
+@pytest.mark.parametrize("d,r", [(64, 0), (64, 32), (80, 40), (96, 16), (40, 24), (128, 8), (6, 4)])
+def test_elements_past_the_rotary_dim_pass_whatever_they_are(dt, interleaved, t, d, r):
+    """Infinities, NaN and -0.0 behind the rotary dim come out as they are, and change nothing else: in the vector
+    kernels (one and two heads a team), in the element-wise one (rows off the 16-byte grid), and through the append."""
+    ops, rng = _ops(), seeded(d + r)
+    hq, hkv = 5, 3
+    table = ops.rope_cos_sin(64, r, device="cuda")
+    pos = dev(rng.integers(0, 64, t).astype(np.int64))
+    slots = torch.randperm(t, device="cuda")
+    for wide in (d, d + 1):
+        x = torch.zeros((t, hq + 2 * hkv, wide), dtype=DT[dt], device="cuda")[..., :d]
+        x.copy_(torch.from_numpy(rng.standard_normal((t, hq + 2 * hkv, d)).astype(np.float32)))
+        plain = x[:, :hq].clone(), x[:, hq:hq + hkv].clone()
+        x[..., r:] = _special(x[..., r:])
+        q, k, v = x[:, :hq], x[:, hq:hq + hkv], x[:, hq + hkv:]
+        kc = torch.zeros((t, 1, hkv, d), dtype=DT[dt], device="cuda")
+        vc = kc.clone()
+        got = *ops.qk_norm_rope(q, k, pos, table, interleaved=interleaved), \
+            ops.rope_paged_kv_append(q, k, v, kc, vc, slots, pos, table, interleaved=interleaved), kc[slots, 0]
+        for out, src, fin in zip(got, (q, k, q, k), plain + plain):
+            assert _same(out[..., r:], src[..., r:])
+            ref, size = rope.norm_rope(host(fin), None, host(pos), host(table), EPS, interleaved)
+            _near(out[..., :r], ref[..., :r], size[..., :r], DT[dt])
+        assert _same(vc[slots, 0], v)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_zeros_keep_their_signs_behind_the_rotary_dim_of_normalised_heads(interleaved):
+    ops = _ops()
+    x = torch.randn((4, 6, 64), device="cuda")
+    x[..., 33::5] = -0.0
+    x[..., 34::5] = 0.0
+    w = torch.ones(64, device="cuda")
+    out, _ = ops.qk_norm_rope(x, x, torch.arange(4, device="cuda"), ops.rope_cos_sin(8, 32, device="cuda"), w, w, EPS, interleaved)
+    zero = x[..., 32:] == 0
+    assert _same(out[..., 32:][zero], x[..., 32:][zero])
