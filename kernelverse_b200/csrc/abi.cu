@@ -71,7 +71,7 @@ __global__ void selftest_wait_kernel(const int4* src, int* out) {
 __global__ void selftest_div_kernel(const float* a, const float* b, float* out, int64_t n) {
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
     const Divisor d = make_divisor(b[i]);
-    if ((i & 2) && fabsf(a[i]) >= d.thresh) {
+    if ((i & 2) && fabsf(a[i]) >= d.thresh && fabsf(a[i]) <= d.limit) {
       const float2 q = f2_unpack(div2_rn_fast(f2_pack(a[i], -a[i]), d));
       out[i] = (q.y == -q.x) ? q.x : __int_as_float(0x7fc00000);   // lanes must agree (NaN otherwise)
     } else {

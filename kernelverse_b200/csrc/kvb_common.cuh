@@ -220,31 +220,33 @@ cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t sme
 // r = a - b*q0 is exact in one FMA and q1 = RN(q0 + r*y) is the round-to-nearest
 // quotient.  The theorem assumes that nothing underflows or overflows in the
 // intermediate steps.  Domain of the fast path: 2^-120 <= b <= 2^120 and
-// max(2^-96, b * 2^-100) <= |a| <= 2^100 * b -- the quantisers always have
-// |a| <= 448 * b because b is the group's amax / 448 (or / 127) or larger.
-// Below the lower bound (zero included, which keeps the quotient's sign) the
-// IEEE division is used; when b is out of range every element of the group is.
+// max(2^-96, b * 2^-100) <= |a| <= 2^100 * b, a finite.  Outside of it (zero included,
+// which keeps the quotient's sign, and every element of a group whose b is out of range)
+// the IEEE division is used: a group's amax / 448 (or / 127) as the scale keeps |a| below
+// 448 * b, but a cache's scale is the caller's, and what it meets may be infinite.
 // A divisor is set up once per quantisation group and reused for every element.
 // tests/test_gpu_numerics.py checks div_rn against CUDA's __fdiv_rn bit for bit.
 struct Divisor {
-  float b, y, thresh;
+  float b, y, thresh, limit;     // the fast path takes thresh <= |a| <= limit
 };
 __device__ __forceinline__ Divisor make_divisor(float b) {
   Divisor d;
   d.b = b;
   d.y = __frcp_rn(b);
   d.thresh = (b >= 0x1p-120f && b <= 0x1p120f) ? fmaxf(0x1p-96f, b * 0x1p-100f) : __int_as_float(0x7f800000);
+  d.limit = fminf(b * 0x1p100f, 0x1.fffffep127f);
   return d;
 }
-// Fast path only: the caller has checked |a| >= d.thresh.
+// Fast path only: the caller knows that d.thresh <= |a| <= d.limit.
 __device__ __forceinline__ float div_rn_fast(float a, const Divisor& d) {
   const float q0 = __fmul_rn(a, d.y);
   const float r = __fmaf_rn(-d.b, q0, a);
   return __fmaf_rn(r, d.y, q0);
 }
 __device__ __forceinline__ float div_rn(float a, const Divisor& d) {
-  if (fabsf(a) < d.thresh) return __fdiv_rn(a, d.b);
-  return div_rn_fast(a, d);
+  const float m = fabsf(a);
+  if (m >= d.thresh && m <= d.limit) return div_rn_fast(a, d);
+  return __fdiv_rn(a, d.b);
 }
 
 // ------------------------------------------------------------------ packed float32 (sm_100a)
@@ -288,7 +290,7 @@ __device__ __forceinline__ uint64_t div2_rn_fast(uint64_t a, const Divisor& d) {
 }
 
 // int8 code: round-half-even of the IEEE float32 quotient x / scale, clamped to +-127.
-// kChecked = false: the caller has verified |x| >= d.thresh for the values passed.
+// kChecked = false: the caller has verified that the values passed are in the fast path's domain.
 template <bool kChecked = true>
 __device__ __forceinline__ int8_t quant_int8(float x, const Divisor& d) {
   float q = rintf(kChecked ? div_rn(x, d) : div_rn_fast(x, d));

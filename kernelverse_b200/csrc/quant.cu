@@ -13,7 +13,7 @@ namespace kvb {
 namespace {
 
 // Packs eight int8 codes of one Vec8 into a 64-bit word (little-endian order); the general
-// path for any divisor (IEEE division below the Markstein threshold, clamp to +-127).
+// path for any divisor (IEEE division outside the Markstein domain, clamp to +-127).
 template <typename T>
 __device__ __forceinline__ uint2 quant8_checked(const Vec8<T>& v, const Divisor& d) {
   float f[8];

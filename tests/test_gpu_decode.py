@@ -381,3 +381,30 @@ def test_fp8_decode_repeated_calls_and_graph_replay():
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(captured, first)
+
+
+@pytest.mark.parametrize("fused", [False, True])
+def test_fp8_writes_saturate_what_is_out_of_range(fused):
+    """Infinities and quotients past float32 are stored as +-448, NaN as NaN, by the write alone and by the decode's."""
+    rng = seeded(12)
+    T, hkv, D = 5, 4, 128
+    sc = np.array([0.005, 1.0, 2.0 ** -125, 2.0 ** 121], np.float32)
+    x = numerics.round_bf16(rng.standard_normal((T, hkv, D)).astype(np.float32))
+    for i, value in enumerate((np.inf, -np.inf, np.nan, 3.3e38, -3.3e38, 1e37)):
+        x.reshape(-1)[2 * i::13] = numerics.round_bf16(np.array([value], np.float32))
+    xt = dev(x, torch.bfloat16)
+    kc = torch.zeros((T, 1, hkv, D), dtype=torch.float8_e4m3fn, device="cuda")
+    vc = torch.zeros_like(kc)
+    if fused:
+        one = torch.ones(T, dtype=torch.int32, device="cuda")
+        table = torch.arange(T, dtype=torch.int32, device="cuda").view(T, 1)
+        _ops().paged_fp8_decode(torch.zeros((T, hkv, D), dtype=torch.bfloat16, device="cuda"), kc, vc, dev(sc), dev(sc), one,
+                                table, k_new=xt, v_new=xt)
+    else:
+        for c in (kc, vc):
+            _ops().paged_fp8_kv_write(xt, c, torch.arange(T, device="cuda"), dev(sc))
+    with np.errstate(all="ignore"):
+        q = np.clip(x / sc[None, :, None], np.float32(-448), np.float32(448))
+    want = np.where(np.isnan(q), np.float32(np.nan), numerics.e4m3_decode(numerics.e4m3_encode(np.nan_to_num(q, nan=0.0))))
+    for c in (kc, vc):
+        np.testing.assert_array_equal(numerics.e4m3_decode(host(c)).reshape(T, hkv, D), want)

@@ -85,3 +85,20 @@ def test_all_mantissas_of_one_binade():
                np.float32(0.7071068), np.float32(448.0 / 127)):
         b = np.full_like(a, bv)
         _assert_same_bits(_run(a, b), a, b)
+
+
+def test_div_out_of_the_fast_domain():
+    """Infinities, NaN, zeros and quotients that overflow or vanish: the IEEE quotient too."""
+    require_gpu()
+    rng = np.random.default_rng(3)
+    a = np.array([np.inf, -np.inf, np.nan, 3.4028235e38, -3.4028235e38, 1e37, -1e37, 1.0, -1.0, 0.0, -0.0, 1e-45, 2.0 ** -126],
+                 np.float32)
+    b = np.array([2.0 ** -149, 2.0 ** -127, 1e-38, 2.0 ** -121, 2.0 ** -120, 1e-30, 2.0 ** -30, 0.005, 1.0, 3.0, 2.0 ** 28,
+                  2.0 ** 120, 2.0 ** 121, 3e38], np.float32)
+    a, b = (x.ravel() for x in np.meshgrid(a, b))
+    n = 1 << 20
+    far = (rng.standard_normal(n) * np.exp2(rng.integers(-140, 127, n))).astype(np.float32)
+    by = np.abs(rng.standard_normal(n) * np.exp2(rng.integers(-140, 127, n))).astype(np.float32) + np.float32(1e-44)
+    with np.errstate(all="ignore"):
+        _assert_same_bits(_run(*(np.repeat(x, 4) for x in (a, b))), np.repeat(a, 4), np.repeat(b, 4))
+        _assert_same_bits(_run(far, by), far, by)

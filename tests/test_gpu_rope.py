@@ -349,3 +349,38 @@ def test_zeros_keep_their_signs_behind_the_rotary_dim_of_normalised_heads(interl
     out, _ = ops.qk_norm_rope(x, x, torch.arange(4, device="cuda"), ops.rope_cos_sin(8, 32, device="cuda"), w, w, EPS, interleaved)
     zero = x[..., 32:] == 0
     assert _same(out[..., 32:][zero], x[..., 32:][zero])
+
+
+def _codes(x, scale):
+    """The value of e4m3(clamp(x / scale, +-448)) in float32; NaN for NaN."""
+    with np.errstate(all="ignore"):
+        q = np.clip(x.astype(np.float32) / scale.astype(np.float32)[None, :, None], np.float32(-448), np.float32(448))
+    out = numerics.e4m3_decode(numerics.e4m3_encode(np.nan_to_num(q, nan=0.0)))
+    return np.where(np.isnan(q), np.float32(np.nan), out)
+
+
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("t", [6, 4000])
+@pytest.mark.parametrize("d,wide", [(64, 64), (20, 20), (64, 65)])
+def test_append_saturates_what_is_out_of_range(dt, t, d, wide):
+    """Infinities and quotients past float32 become +-448 and NaN stays NaN, for scales of a cache's size and for the
+    smallest and largest: vectors of eight and of four, one and two heads a team, and the element-wise kernel."""
+    ops, rng = _ops(), seeded(d + t)
+    scale = np.array([0.005, 1.0, 2.0 ** -125, 1e-38, 2.0 ** -120, 2.0 ** 120, 2.0 ** 125], np.float32)
+    hkv = len(scale)
+    x = torch.zeros((t, 2 * hkv, wide), dtype=DT[dt], device="cuda")[..., :d]
+    x.copy_(torch.from_numpy(rng.standard_normal((t, 2 * hkv, d)).astype(np.float32)))
+    top = torch.finfo(DT[dt]).max
+    flat = torch.arange(x.numel(), device="cuda").view(x.shape)
+    for i, value in enumerate((float("inf"), float("-inf"), float("nan"), top, -top, top / 16, 0.0, -0.0)):
+        x[flat % 17 == 2 * i] = value
+    k, v = x[:, :hkv], x[:, hkv:]
+    kc = torch.zeros((t, 1, hkv, d), dtype=torch.uint8, device="cuda")
+    vc = kc.clone()
+    slots = torch.randperm(t, device="cuda")
+    sc = dev(scale)
+    ops.rope_paged_kv_append(k, k, v, kc, vc, slots, torch.zeros(t, dtype=torch.int64, device="cuda"),
+                             torch.zeros((1, 0), device="cuda"), sc, sc)
+    for cache, src in ((kc, k), (vc, v)):
+        got = numerics.e4m3_decode(cache[slots, 0].cpu().numpy())
+        np.testing.assert_array_equal(got, _codes(host(src.contiguous()), scale))
