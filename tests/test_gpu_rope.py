@@ -384,3 +384,28 @@ def test_append_saturates_what_is_out_of_range(dt, t, d, wide):
     for cache, src in ((kc, k), (vc, v)):
         got = numerics.e4m3_decode(cache[slots, 0].cpu().numpy())
         np.testing.assert_array_equal(got, _codes(host(src.contiguous()), scale))
+
+
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("hq,hkv,d,r", [(5, 3, 64, 64), (4, 1, 80, 40), (7, 2, 20, 16), (6, 3, 128, 64)])
+def test_long_inputs_two_heads_a_team(dt, interleaved, hq, hkv, d, r):
+    """Long inputs give a team two heads: teams with a query and a key head, a key and a value head, and one head only;
+    vectors of eight and of four; partial rotation; positions out of range keep to their own tokens."""
+    from kernelverse_b200 import _lib
+    t = 10000
+    _check(d + hq, t, hq, hkv, d, r, dt, interleaved, True)
+    _append(d + hkv, t, hq, hkv, d, r, 16, dt, dt, interleaved, False, padded=900)
+    _append(d + hkv, t, hq, hkv, d, r, 16, dt, "e4m3", interleaved, True)
+    ops = _ops()
+    q, k, _, pos, table = _case(1, t, hq, hkv, d, r, dt)
+    qw, kw = _weights(1, d, dt)
+    want = ops.qk_norm_rope(q, k, pos, table, qw, kw, EPS, interleaved)
+    bad = pos.clone()
+    bad[::7], bad[3::70] = 500, -1
+    out = (bad < 0) | (bad >= 500)
+    assert _lib.lib().kvb_device_status(1) == 0
+    got = ops.qk_norm_rope(q, k, bad, table, qw, kw, EPS, interleaved)
+    assert _lib.lib().kvb_device_status(1) == 2
+    for g, w in zip(got, want):
+        assert g[out].isnan().all() and torch.equal(g[~out], w[~out])
