@@ -448,7 +448,12 @@ KVB_API size_t kvb_paged_prefill_attention_workspace_size(int head_dim);
  * were.  max_seq_len >= every seq_len.  A request whose lengths lie outside the tensors is skipped
  * (bit 2 of kvb_device_status); a block-table entry out of range counts as zero keys and values and
  * sets bit 1.  Float32 softmax state; parts of one row are joined in a fixed order, so equal inputs
- * give equal outputs.  head_dim a multiple of 8, at most 128.  workspace: >=
+ * give equal outputs.  The products' operands: the weights exp(s - max) are rounded to bfloat16 over
+ * bfloat16 caches (on mma.sync: for bfloat16 queries), otherwise to float16; over KVB_E4M3 the tcgen05
+ * kernel holds q as float16 times a power of two for each row, which keeps elements down to 2^-14 of the
+ * row's largest in full; float32 operands go as three TF32 products.  A value that is not finite reaches
+ * the queries that see it and may reach queries before it (their weight is 0, and 0 * inf is NaN).
+ *  head_dim a multiple of 8, at most 128.  workspace: >=
  * kvb_paged_prefill_attention_workspace_size() bytes, 256-byte aligned, not shared with a launch that
  * may run at the same time.
  */

@@ -60,7 +60,9 @@ __device__ __forceinline__ bool pg_request(const PagedArgs& a, int b, PgRequest&
 }
 
 // sum over t in [0, n) of floor((b + s t) / m), b >= 0, s, m > 0, all numerators below 2^31
-// (the Euclid-like recursion on (s, m)).
+// (what s and b hold of whole m's in closed form, then the lattice points below the line counted from the
+// other axis, which swaps s and m as Euclid's algorithm does: Graham, Knuth, Patashnik, Concrete
+// Mathematics, 2nd ed., section 3.5).
 __host__ __device__ __forceinline__ int64_t pg_floor_sum(uint32_t n, uint32_t m, uint32_t s, uint32_t b) {
   int64_t ans = 0;
   while (n > 0) {
@@ -121,7 +123,7 @@ struct PgShare {
 // Fills `s` (shared memory) for CTA `cta` of `grid`.  All NT threads call it; it ends with a barrier.
 template <int NT>
 __device__ __forceinline__ void pg_share(const PagedArgs& a, const PgTiles& tiles, int cta, int grid, PgShare* s,
-                                         int64_t* scan /* NT / 32 + 1 */, unsigned int* status) {
+                                         int64_t* scan /* NT / 32 */, unsigned int* status) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   constexpr int NW = NT / 32;
   int64_t mine = 0;                                // requests tid, tid + NT, ...: for the total

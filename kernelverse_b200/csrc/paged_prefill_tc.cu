@@ -25,9 +25,13 @@
 // TMA fills with zeros; the rows past the last token inside its page are zeroed in shared memory.
 // e4m3: a row of Q is scaled by a power of two that brings its largest element to [1, 2), so float16
 // holds it whatever bfloat16's range had; P is float16 too.
-// What bounds it: for long chunks the chains' hand-overs and the operands of S in shared memory (2048 new
-// tokens of 16384, 32 + 8 heads of 128, bf16: 520-540 us, 0.58 of the bf16 rate; 4 x 512 of 4096 over
-// codes 180-190 us); for decoding over 16-bit caches HBM (64 sequences of 4352 tokens: 197 us, 5.8 TB/s).
+// What bounds it: for long chunks two things that have to overlap, the products (S at N = 64 takes 48 cycles
+// where 32 would do) and the exponentials (512 cycles for the 128 x 64 scores that a chain's products take
+// ~640 for): 2048 new tokens of 16384, 32 + 8 heads of 128, bf16: 530 us, 0.58 of the bf16 rate, tensor pipe
+// 53 % and exponentials 59 % of the time.  4 x 512 of 4096 over codes: 185-190 us, those 33 % and 37 %: four
+// warps convert every K and V tile in one order.  Decoding over 16-bit caches: HBM (64 sequences of 512 to
+// 8192 tokens: 169 us, 5.2 TB/s).  At 128 registers a thread the kernels over codes spill (276 to 312 bytes
+// stored), those over 16-bit caches 48.
 // Every wait is bounded: by a time limit where one hand-over is waited for, by the limit since the last copy was
 // issued where whole items are (a page tail at the end of a share, query rows behind few-row items); on a timeout the roles stop, the producer waits for its own copies,
 // the MMA lanes for their MMAs, and the CTA frees its TMEM before exiting.
@@ -177,8 +181,9 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 // K and V are their A operands, straight from the tile (codes turned into float16 on the way: no operand tile is
 // written), Q^T and P^T the B operands, and P^T is S^T's fragment transposed.  What a row needs of a head is one
 // pass over the keys, so nothing but the bytes counts; the tcgen05 products take 128 rows and two hand-overs a
-// tile for the same (a decoding step of 64 sequences of up to 8192 tokens: 226 us with them, 145 like this; 16-bit
-// caches gained nothing, 197 and 201 us: there the bytes count either way).
+// tile for the same (a decoding step of 64 sequences of up to 8192 tokens: 226 us with them, 147 like this, 3.0 TB/s;
+// 16-bit caches gained nothing, 197 and 201 us: there the bytes count either way).  What bounds it is latency: eight
+// warps an SM carry the whole chain of loads, conversions and products (issue slots 29 % used, DRAM 36 %).
 template <typename T, class Join>
 __device__ __forceinline__ bool thin_item(const PagedArgs& a, const PgItem& it, const PcItem& g, uint8_t* smem, uint64_t* full,
                                           uint64_t* empty, uint32_t u, float* ml_s, Join& join) {
@@ -1105,7 +1110,9 @@ int launch_pc(const CUtensorMap& mk, const CUtensorMap& mv, const PagedArgs& a, 
 
 // Whether the tcgen05 kernel takes the case: 16-bit queries, head_dim a multiple of 16 in [64, 128], and
 // pages that a tile of 128 keys is cut into at most 32 boxes by (a box lies in one page, its rows start on
-// the 128-byte grid that TMA wants).
+// the 128-byte grid that TMA wants).  It takes them at every length.  mma.sync kernel / this one, 32 + 8 heads of
+// 128, bf16: 2 x 4 of 1000 tokens 17.8 / 16.7 us (over codes 20.3 / 15.4; head_dim 64 14.7 / 15.1), 8 x 1 of
+// 500 20.0 / 18.9, 4 x 256 of 256 47.9 / 41.8, 64 x 1 of 4000 433 / 181; one prompt of 64 tokens 10.5 / 16.7.
 bool paged_prefill_tc_takes(const PagedArgs& a, int q_dtype, int cache_dtype) {
   const int cs = cache_dtype == KVB_E4M3 ? 1 : 2;
   return (q_dtype == KVB_BF16 || q_dtype == KVB_F16) && a.D % 16 == 0 && a.D >= 64 && a.D <= 128 && a.bs % 4 == 0 &&

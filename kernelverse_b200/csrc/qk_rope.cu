@@ -10,11 +10,13 @@
 // e4m3(clamp(y / scale[h], +-448)), quantised from the float32 value with the correctly rounded
 // quotient.
 //
-// What bounds it: HBM for prompts (each element is read once and written once), the launch for
-// decode steps.  A head is held by a team of a few lanes, each with the two V-element vectors
-// whose elements pair up, so the rotation needs no exchange and the norm one shuffle tree; a lane
-// keeps the same element range for every head it serves, so cos, sin and the weights are loaded
-// once per token and lane.
+// Each element is read once and written once.  What bounds it: the launch for decode steps; for
+// prompts latency (3.7 of 6.55 TB/s; DRAM 31 %, issue slots 60 %: a block lives for one round of
+// loads, so none of the next heads' are in flight while it computes).  A head is held by a team of
+// a few lanes, each with the two V-element vectors whose elements pair up, so the rotation needs no
+// exchange and the norm one shuffle tree; a lane keeps the same element range for every head it
+// serves, so cos and sin are loaded once per token and lane; the weights are loaded for each head,
+// from L1.
 #include <type_traits>
 
 #include "kvb_common.cuh"
@@ -418,7 +420,7 @@ cudaError_t launch_rope(const RopeArgs& a, cudaStream_t st) {
   while ((1 << llanes) < pairs) ++llanes;
   // Two heads a team once that still gives every SM its blocks: cos and sin are then loaded once for both
   // and four vector loads are in flight per lane (8192 tokens of 32 + 8 heads of 128, bf16, normalised:
-  // 45.9 us, 3.7 TB/s; one head 53.1, four 50.6).
+  // 46.5 us, 3.7 TB/s; one head 53.1, four 50.6).
   const int64_t per = kRopeThreads >> llanes;
   const bool many = a.tokens * ((heads + kRopeHeads - 1) / kRopeHeads) >= 148LL * kRopeBlocks * per;
   const int64_t groups = many ? (heads + kRopeHeads - 1) / kRopeHeads : heads;

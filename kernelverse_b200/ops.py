@@ -631,12 +631,17 @@ def paged_prefill_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     position.  One token a request is a decode step, a few check drafted tokens, many prefill a prompt;
     a batch may mix them.  Caches [num_blocks, block_size, Hkv, D] of q's dtype, or e4m3 codes
     (float8_e4m3fn or uint8) with float32 ``k_scale`` / ``v_scale`` [Hkv]; block_table int32 [B, max_blocks].
-    Logits are scaled by ``scale`` (default D^-0.5); float32 softmax.  ``max_seq_len`` (default: what the
-    block table holds) bounds every seq_len.
+    Logits are scaled by ``scale`` (default D^-0.5).  Softmax in float32, its weights rounded to bfloat16 or
+    float16 for the product with V (float32 inputs: products of three TF32 terms).
+    ``max_seq_len`` (default: what the block table holds, and no more) bounds every seq_len.
 
     Returns [total_q, Hq, D] in q's dtype (``out`` when given), and with ``return_lse`` the natural-log
-    sums of exp [total_q, Hq] float32.  A query that sees no key (q_len > seq_len) gives 0 and -inf; rows
-    past the last request are left as they were.  Equal inputs give equal outputs."""
+    sums of exp [total_q, Hq] float32.  A query that sees no key (q_len > seq_len) gives 0 and -inf.  Rows that no
+    request owns keep what ``out`` held (without ``out``, and in the log-sum-exps, they are not set).  A value that
+    is not finite may also reach queries of its chunk that stand before it.  Equal inputs give equal outputs.
+
+    A batch of nothing but single tokens is faster with :func:`paged_fp8_decode` (e4m3 codes) or
+    :func:`paged_attention_v1`, unless it is a few long sequences: this operator splits those further."""
     what = "paged_prefill_attention"
     dev = _device_of(what, q, k_cache, v_cache, qo_indptr, seq_lens, block_table, k_scale, v_scale, out)
     if dev != _current_device():
